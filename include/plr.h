@@ -183,6 +183,124 @@ int plr_loss_grad_noalloc(int device_id, void* hip_stream, const double* dX,
                           const double* dy, int64_t n, int64_t d, int64_t ldx,
                           const double* dtheta, double* dout, unsigned flags);
 
+/* ---- 4-bit matrices and dropout ------------------------------------------
+ * No counterpart in the reference, whose samples are doubles throughout.
+ *
+ * Microscaled 4-bit floating point: 32 consecutive values of a row share a
+ * power of two 2^(s - 127) (s: one byte), a value is a 4-bit code (sign, two
+ * exponent bits, a mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two codes to a
+ * byte with the even column in the low half: 17/32 of a byte per value.  s is
+ * floor(log2 of the block's largest magnitude) - 2 + 127, within 0..254; a
+ * value is rounded to the nearest code, ties to the even one, and saturates
+ * at 6.  A block that holds a NaN or an infinity gets s = 255 and stands for
+ * NaN throughout.  A matrix is an array of code rows (pitch in bytes, a
+ * multiple of 16) and an array of scale rows (pitch in bytes).
+ *
+ * Dropout: a matrix's value in column j of row i is kept with probability
+ * 1 - rate, where a 16-bit random word reaches rint(rate * 65536), and then
+ * multiplied by 65536 / (65536 - rint(rate * 65536)).  The word is a function
+ * of (seed, step, row0 + i, j) alone (Philox4x32-10 with the counter
+ * (j / 8, row low, row high, step) under the key seed; word j % 8 of its 128
+ * bits), so no mask is stored: the call for the gradient names the same
+ * plr_dropout and meets the same mask.
+ *
+ * The calls below take DEVICE pointers, enqueue kernels on `hip_stream` (a
+ * hipStream_t; NULL = the default stream) and return without waiting.  They
+ * allocate nothing, keep nothing between calls and leave the caller's current
+ * device as they found it; the first call of any of them on a device looks
+ * its properties up, which a caller that captures the stream has happen
+ * before the capture begins.  Calls may overlap as far as their outputs (and
+ * workspaces) are apart.  Errors are described by plr_last_error(NULL). */
+
+/* element types of device matrices */
+#define PLR_F64 0u
+#define PLR_F32 1u
+#define PLR_BF16 2u
+#define PLR_F16 3u
+
+typedef struct plr_dropout {
+  double rate;    /* 0 <= rate <= 65535/65536 */
+  uint64_t seed;
+  int64_t row0;   /* the matrix's first row, >= 0: a worker's or a batch's rows keep the mask
+                     they have in the whole matrix */
+  uint32_t step;  /* a new mask per step under the same seed */
+} plr_dropout;
+
+/* Bytes per row that the product below needs of a matrix of d columns: codes
+ * and scales of whole 128-column chunks, ceil(d / 128) * 64 and * 4. */
+int64_t plr_mxfp_code_pitch(int64_t d);
+int64_t plr_mxfp_scale_pitch(int64_t d);
+
+#define PLR_MXFP_TRANSPOSE 1u
+
+/* n x d values of `type` at a row pitch of ldx values -> 4 bits.  Codes go to
+ * dcodes (16-byte aligned, row pitch ldc bytes, a multiple of 16 that holds
+ * 16 bytes per started block of 32 columns), scale bytes to dscales (pitch
+ * lds >= the number of blocks).  The last chunk of 128 columns is written to
+ * its end as far as the pitches reach, with zeros behind column d; bytes
+ * behind it are left as they were.
+ *   PLR_MXFP_TRANSPOSE  quantises the transpose: d rows of n columns, blocks
+ *        along the columns of x -- the operand a gradient's product needs.
+ *   drop (nullable)  values the mask drops count as 0; kept ones are NOT
+ *        multiplied (a power of two is no home for 65536 / (65536 - t): pass
+ *        it as alpha to the product).  Rows and columns are those of x, in
+ *        either orientation. */
+int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned type, int64_t n,
+                      int64_t d, int64_t ldx, unsigned flags, const plr_dropout* drop,
+                      uint8_t* dcodes, int64_t ldc, uint8_t* dscales, int64_t lds);
+
+/* The n x d values a 4-bit matrix stands for, rounded once to `type`. */
+int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, int64_t ldc,
+                        const uint8_t* dscales, int64_t lds, int64_t n, int64_t d, void* dout,
+                        unsigned type, int64_t ldo);
+
+/* C[i][j] = alpha * sum_k A[i][k] * B[j][k], A of m rows and B of n rows of k
+ * columns in 4 bits, the sums in 32 bits, C of `type` (PLR_F32, PLR_BF16 or
+ * PLR_F16) at a row pitch of ldc values.  The scores of m samples under n
+ * coefficient vectors, next to plr_predict_linear's one; with
+ * PLR_MXFP_TRANSPOSE operands also both gradients of such a product:
+ * dA = dC B as quantise(dC) . quantise(B, transposed) and dB = dC^T A as
+ * quantise(dC, transposed) . quantise(A, transposed).
+ * Code pitches are multiples of 64 and at least plr_mxfp_code_pitch(k), scale
+ * pitches multiples of 4 and at least plr_mxfp_scale_pitch(k); codes between
+ * column k and the end of its chunk must be 0 and their scales not 255 (as
+ * plr_mxfp_quantize leaves them).  da and db 16-byte, dsa and dsb 4-byte
+ * aligned.
+ *   drop (nullable)  dropout of C: a gradient with respect to a dropped A.
+ *   workspace  plr_mxfp_matmul_workspace(m, n, k) bytes of device memory,
+ *        16-byte aligned, used while the call's kernels run (0: may be NULL). */
+int64_t plr_mxfp_matmul_workspace(int64_t m, int64_t n, int64_t k);
+int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64_t k,
+                    const uint8_t* da, int64_t lda, const uint8_t* dsa, int64_t ldsa,
+                    const uint8_t* db, int64_t ldb, const uint8_t* dsb, int64_t ldsb, double alpha,
+                    const plr_dropout* drop, void* dc, unsigned type, int64_t ldc, void* workspace,
+                    int64_t workspace_bytes);
+
+/* out = dropout of x, both n x d values of `type`; the same call on the
+ * gradient of out gives the gradient of x.  A dropped value is 0 whatever it
+ * was.  In place where dout == dx and ldo == ldx. */
+int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned type, int64_t n,
+                      int64_t d, int64_t ldx, void* dout, int64_t ldo, const plr_dropout* drop);
+
+/* Hold the resident shard in 4 bits from now on (the doubles are released):
+ * every pass then computes, in 64 bits, on the values the codes stand for, and
+ * reads 17/32 of a byte per value instead of 8.  A constant first column that
+ * is not stored ("first_column_is_one") stays exact.  plr_get_data returns the
+ * rounded values; plr_set_data_chunk is refused until the next plr_set_data /
+ * plr_alloc_data, which starts a shard of doubles again. */
+int plr_pack_data(plr_ctx* ctx);
+
+/* Dropout of the shard's values in the passes that make a gradient
+ * (plr_loss_grad, plr_dgd_delta, plr_dgd_delta_linear, plr_train_dgd) over a
+ * shard held in 4 bits, from now on; NULL: none.  Column 0 of the mask is the
+ * first stored column (a constant first column that is not stored is never
+ * dropped).  plr_train_dgd's round r uses step + r; the other calls use step
+ * as given, so a caller names a new one every round.  The loss of such a pass
+ * is that of the dropped values; plr_calc_loss and plr_predict never drop.
+ * On a shard of doubles these passes fail with PLR_ERR_UNSUPPORTED while
+ * dropout is set (plr_dropout_apply and plr_loss_grad_noalloc serve there). */
+int plr_set_dropout(plr_ctx* ctx, const plr_dropout* drop);
+
 /* Block until everything this context (and the device) was asked to do has
  * finished.  The compute entry points already return drained; this is the
  * explicit fence benchmarks put on both sides of a timed region. */
@@ -269,7 +387,8 @@ const char* plr_kernel_info(const plr_ctx* ctx);
 
 /* Context-owned message of the last error ("" if none); never freed.
  * plr_last_error(NULL) describes the last failure of a call that takes no
- * context (plr_create, plr_loss_grad_noalloc). */
+ * context (plr_create, plr_loss_grad_noalloc, the plr_mxfp_* calls and
+ * plr_dropout_apply). */
 const char* plr_last_error(const plr_ctx* ctx);
 
 const char* plr_version(void);

@@ -50,7 +50,8 @@ def hipcc():
 def build_libplr():
     """HIP kernels + C ABI -> paracel_amd/libplr.so"""
     out = os.path.join(_HERE, "libplr.so")
-    _run_hipcc([hipcc()] + HIPCC_FLAGS + ["-o", out, os.path.join(_HERE, "csrc", "plr_capi.hip")])
+    _run_hipcc([hipcc()] + HIPCC_FLAGS + ["-o", out, os.path.join(_HERE, "csrc", "plr_capi.hip"),
+                os.path.join(_HERE, "csrc", "plr_ops.hip")])
     return out
 
 

@@ -16,6 +16,25 @@ PLR_LOSS_SQUARED = 3
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
+PLR_F64, PLR_F32, PLR_BF16, PLR_F16 = range(4)
+PLR_MXFP_TRANSPOSE = 1
+
+
+class Dropout(C.Structure):
+    """plr_dropout: the mask is a function of (seed, step, row0 + row, column)."""
+
+    _fields_ = [("rate", C.c_double), ("seed", C.c_uint64), ("row0", C.c_int64),
+                ("step", C.c_uint32)]
+
+    def __init__(self, rate, seed, step=0, row0=0):
+        super().__init__(rate, seed, row0, step)
+
+    @property
+    def scale(self):
+        """What kept values are multiplied by: the rate is taken in steps of 2^-16."""
+        return 65536.0 / (65536 - round(self.rate * 65536))
+
+
 # every symbol include/plr.h declares: (name, restype, argtypes)
 _dp = C.POINTER(C.c_double)
 _i64p = C.POINTER(C.c_int64)
@@ -38,6 +57,22 @@ SYMBOLS = [
     ("plr_predict_linear", C.c_int, [_ctx, _dp, _dp]),
     ("plr_loss_grad_noalloc", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                         C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_uint]),
+    ("plr_mxfp_code_pitch", C.c_int64, [C.c_int64]),
+    ("plr_mxfp_scale_pitch", C.c_int64, [C.c_int64]),
+    ("plr_mxfp_quantize", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_uint, C.c_int64, C.c_int64,
+                                    C.c_int64, C.c_uint, C.POINTER(Dropout), C.c_void_p, C.c_int64,
+                                    C.c_void_p, C.c_int64]),
+    ("plr_mxfp_dequantize", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                      C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_uint,
+                                      C.c_int64]),
+    ("plr_mxfp_matmul_workspace", C.c_int64, [C.c_int64, C.c_int64, C.c_int64]),
+    ("plr_mxfp_matmul", C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64] +
+     [C.c_void_p, C.c_int64] * 4 + [C.c_double, C.POINTER(Dropout), C.c_void_p, C.c_uint, C.c_int64,
+                                    C.c_void_p, C.c_int64]),
+    ("plr_dropout_apply", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_uint, C.c_int64, C.c_int64,
+                                    C.c_int64, C.c_void_p, C.c_int64, C.POINTER(Dropout)]),
+    ("plr_pack_data", C.c_int, [_ctx]),
+    ("plr_set_dropout", C.c_int, [_ctx, C.POINTER(Dropout)]),
     ("plr_synchronize", C.c_int, [_ctx]),
     ("plr_set_timing", C.c_int, [_ctx, C.c_int]),
     ("plr_set_option", C.c_int, [_ctx, C.c_char_p, C.c_int64]),
@@ -103,6 +138,62 @@ def loss_grad_noalloc(dX, dy, n, d, ldx, dtheta, dout, flags=PLR_LOSS_REFERENCE,
     rc = lib.plr_loss_grad_noalloc(int(device), C.c_void_p(stream), C.c_void_p(dX),
                                    C.c_void_p(dy), n, d, ldx, C.c_void_p(dtheta),
                                    C.c_void_p(dout), flags)
+    if rc != 0:
+        raise PlrError(rc, lib.plr_last_error(None).decode())
+
+
+def _ref(drop):
+    return C.byref(drop) if drop is not None else None
+
+
+def mxfp_code_pitch(d):
+    """Bytes of code per row that the product needs of a matrix of d columns."""
+    return load_library().plr_mxfp_code_pitch(d)
+
+
+def mxfp_scale_pitch(d):
+    """Scale bytes per row that the product needs of a matrix of d columns."""
+    return load_library().plr_mxfp_scale_pitch(d)
+
+
+def mxfp_quantize(dx, dtype, n, d, ldx, dcodes, ldc, dscales, lds, transpose=False, drop=None,
+                  device=0, stream=None):
+    """plr_mxfp_quantize on raw DEVICE addresses (ints), as loss_grad_noalloc takes them."""
+    lib = load_library()
+    rc = lib.plr_mxfp_quantize(device, stream, dx, dtype, n, d, ldx,
+                               PLR_MXFP_TRANSPOSE if transpose else 0, _ref(drop), dcodes, ldc,
+                               dscales, lds)
+    if rc != 0:
+        raise PlrError(rc, lib.plr_last_error(None).decode())
+
+
+def mxfp_dequantize(dcodes, ldc, dscales, lds, n, d, dout, dtype, ldo, device=0, stream=None):
+    """plr_mxfp_dequantize on raw DEVICE addresses."""
+    lib = load_library()
+    rc = lib.plr_mxfp_dequantize(device, stream, dcodes, ldc, dscales, lds, n, d, dout, dtype, ldo)
+    if rc != 0:
+        raise PlrError(rc, lib.plr_last_error(None).decode())
+
+
+def mxfp_matmul_workspace(m, n, k):
+    """Bytes of workspace mxfp_matmul needs for these sizes."""
+    return load_library().plr_mxfp_matmul_workspace(m, n, k)
+
+
+def mxfp_matmul(m, n, k, da, lda, dsa, ldsa, db, ldb, dsb, ldsb, dc, dtype, ldc, alpha=1.0,
+                drop=None, workspace=None, workspace_bytes=0, device=0, stream=None):
+    """plr_mxfp_matmul on raw DEVICE addresses: C = alpha * A B^T, A and B in 4 bits."""
+    lib = load_library()
+    rc = lib.plr_mxfp_matmul(device, stream, m, n, k, da, lda, dsa, ldsa, db, ldb, dsb, ldsb, alpha,
+                             _ref(drop), dc, dtype, ldc, workspace, workspace_bytes)
+    if rc != 0:
+        raise PlrError(rc, lib.plr_last_error(None).decode())
+
+
+def dropout_apply(dx, dtype, n, d, ldx, dout, ldo, drop, device=0, stream=None):
+    """plr_dropout_apply on raw DEVICE addresses (forward, or backward on the gradient)."""
+    lib = load_library()
+    rc = lib.plr_dropout_apply(device, stream, dx, dtype, n, d, ldx, dout, ldo, _ref(drop))
     if rc != 0:
         raise PlrError(rc, lib.plr_last_error(None).decode())
 
@@ -192,6 +283,14 @@ class Plr:
         y = np.empty(nrows)
         self._check(self._lib.plr_get_data(self._h, row0, nrows, _p(X), d, _p(y)))
         return X, y
+
+    def pack_data(self):
+        """Hold the resident shard in 4 bits from now on (plr_pack_data)."""
+        self._check(self._lib.plr_pack_data(self._h))
+
+    def set_dropout(self, drop):
+        """Dropout (a Dropout, or None for none) of the gradient passes over a packed shard."""
+        self._check(self._lib.plr_set_dropout(self._h, _ref(drop)))
 
     @property
     def shape(self):

@@ -5,6 +5,7 @@
 #include "../../include/plr.h"
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -18,7 +19,9 @@
 #include <vector>
 
 #include "plr_csv.hpp"
+#include "plr_internal.hpp"
 #include "plr_kernels.hpp"
+#include "plr_packed.hpp"
 #include "plr_plan.hpp"
 
 struct plr_ctx;
@@ -111,6 +114,7 @@ static_assert(plr_plan::kTeamMinNch == 7 && plr_plan::kTeamNch == 8 &&
                   plr_plan::kTeamWaves == plr::kTeamWaves,
               "one team kernel set per chunk count");
 constexpr int64_t kHostPredictCols = 192;  // from this pitch on predictions go straight to host
+constexpr int64_t kHostPredictColsPacked = 2048;
 // Results watched for by the host thread (results_arrived): finishing kernels of
 // up to 64 blocks (1024 columns), for at most 20 ms -- longer than any pass over
 // a shard that fits the device -- before the thread waits for the stream instead.
@@ -209,7 +213,29 @@ int g_na_num_cu[kNaMaxDevices] = {};
 int g_na_occ[kNaMaxDevices][kNaMaxPitch / plr::kChunkCols + 1] = {};
 std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 
+// Shard held in 4 bits: kernel instances [dropout].  A row of up to kPackedFused blocks is read
+// once; wider ones go in column pieces of kPackedPiece blocks, in two sweeps.
+typedef void (*packed_fn)(plr::PackedArgs);
+constexpr int kPR = plr::kPackedRows;
+const packed_fn kPackedGrad[2] = {plr::packed_pass<true, false, plr::kPassFused, kPR>,
+                                  plr::packed_pass<true, true, plr::kPassFused, kPR>};
+const packed_fn kPackedEval = plr::packed_pass<false, false, plr::kPassFused, kPR>;
+const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, kPR>,
+                                 plr::packed_pass<false, true, plr::kPassDot, kPR>};
+const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, kPR>,
+                                  plr::packed_pass<true, true, plr::kPassAxpy, kPR>};
+constexpr int kPackedFused = 512, kPackedPiece = 256;
+
 }  // namespace
+
+int plr_fail_without_context(int code, const char* msg) {
+  try {
+    std::lock_guard<std::mutex> lock(g_err_mutex);
+    g_create_error = msg;
+  } catch (...) {
+  }
+  return code;
+}
 
 struct plr_ctx {
   int device = 0;
@@ -300,6 +326,16 @@ struct plr_ctx {
   int done_blocks = 0;          // > 0: the pass just enqueued reports through h_done
   bool opt_poll_results = true; // plr_set_option("poll_results")
 
+  // the shard in 4 bits (plr_pack_data): dX is released then
+  bool packed = false;
+  uint8_t* d_codes = nullptr;     // n x row_blocks * 16 bytes
+  uint8_t* d_scales = nullptr;    // n x row_blocks
+  int64_t row_blocks = 0;
+  int packed_threads = 0;
+  bool packed_sweeps = false;     // too wide for one read: column pieces, two sweeps
+  bool drop_on = false;           // plr_set_dropout
+  plr_dropout drop = {0., 0, 0, 0};
+
   double last_ms = 0., sum_ms = 0.;
   int64_t launches = 0;
   bool timing = true;           // record the two events around the streaming kernels
@@ -337,6 +373,12 @@ void free_shape(plr_ctx* c) {
   (void)hipSetDevice(c->device);
   release_upload_staging(c);
   if (c->dX) (void)hipFree(c->dX);
+  if (c->d_codes) (void)hipFree(c->d_codes);
+  if (c->d_scales) (void)hipFree(c->d_scales);
+  c->d_codes = c->d_scales = nullptr;
+  c->packed = c->packed_sweeps = false;
+  c->row_blocks = 0;
+  c->packed_threads = 0;
   if (c->dy) (void)hipFree(c->dy);
   if (c->d_theta) (void)hipFree(c->d_theta);
   if (c->d_part_g) (void)hipFree(c->d_part_g);
@@ -552,6 +594,52 @@ int plan_shape(plr_ctx* c, int64_t n, int64_t d) {
   return PLR_OK;
 }
 
+// Threads of a workgroup for pieces of `blocks` blocks: 256 or 512, whichever leaves fewer idle.
+int packed_workgroup(int blocks) {
+  if (blocks > 256) return 512;
+  return (512 / blocks) > 2 * (256 / blocks) ? 512 : 256;
+}
+
+size_t packed_lds(int threads, int blocks) {
+  const size_t slots = (size_t)(threads / blocks);
+  return std::max((size_t)threads * 8, slots * kPR * ((size_t)blocks + 1)) * sizeof(double);
+}
+
+// Workgroup and persistent grid of the passes over n rows of dcols columns held in 4 bits.
+int plan_packed(plr_ctx* c, int64_t n) {
+  c->row_blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
+  c->pitch = c->theta_len = c->row_blocks * plr_mx::kBlockCols;
+  c->packed_sweeps = c->row_blocks > kPackedFused;
+  c->var = &kBlockShape;  // unused by this path, kept non-null
+  c->nch_rt = 1;
+  const int blocks = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
+  c->packed_threads = packed_workgroup(blocks);
+  int occ = 1 << 30;
+  const packed_fn used[] = {
+      c->packed_sweeps ? kPackedDot[0] : kPackedGrad[0], c->packed_sweeps ? kPackedDot[1] : kPackedGrad[1],
+      c->packed_sweeps ? kPackedAxpy[0] : kPackedEval, c->packed_sweeps ? kPackedAxpy[1] : kPackedEval};
+  for (packed_fn f : used) {
+    int o = 0;
+    PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(
+                   &o, reinterpret_cast<const void*>(f), c->packed_threads,
+                   packed_lds(c->packed_threads, blocks)));
+    occ = std::min(occ, o);
+  }
+  if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
+  const int64_t tiles = ceil_div(n, (int64_t)(c->packed_threads / blocks) * kPR);
+  c->grid = c->grid_nograd =
+      (int)std::max<int64_t>(1, std::min<int64_t>(tiles, (int64_t)c->num_cu * occ));
+  char b[256];
+  snprintf(b, sizeof b,
+           "packed_pass<R=%d> 4-bit shard, %lld blocks of 32 columns per row%s, %d rows side by side, "
+           "grid=%d x %d threads (occupancy %d blocks/CU, %d CUs)",
+           kPR, (long long)c->row_blocks, c->packed_sweeps ? " in pieces of 256, two sweeps" : "",
+           c->packed_threads / blocks, c->grid, c->packed_threads, occ, c->num_cu);
+  c->info = b;
+  if (c->bias) c->info += "; first column constant 1, not stored";
+  return PLR_OK;
+}
+
 // The rows of an n x d shard: layout and kernel variant for that shape, then X
 // (with the slack the kernels may read past the last row) and y.
 int alloc_rows(plr_ctx* c, int64_t n, int64_t d, bool zero_fill) {
@@ -625,7 +713,7 @@ int alloc_workspace(plr_ctx* c) {
     c->zstride = ceil_div(ceil_div(std::max<int64_t>(n, 1), c->nteams), plr::kWave) * plr::kWave;
     PLR_HIP(c, hipMalloc(&c->d_zparts, (size_t)c->zstride * c->nteams * c->team_blocks *
                                            plr::kTeamWaves * sizeof(double)));
-  } else if (c->blocked && n > 0) {
+  } else if ((c->blocked || c->packed_sweeps) && n > 0) {
     PLR_HIP(c, hipMalloc(&c->d_z, (size_t)n * sizeof(double)));
     PLR_HIP(c, hipMalloc(&c->d_res, (size_t)n * sizeof(double)));
   }
@@ -683,6 +771,71 @@ int upload_rows(plr_ctx* c, int64_t row0, int64_t nrows, const double* X,
 
 enum PassKind { kPassGrad, kPassDelta, kPassLoss, kPassPredict, kPassPredictLinear };
 
+// The streaming kernels of a pass over a shard held in 4 bits.  *loss_parts: how many partial
+// losses they leave.
+int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, int* loss_parts) {
+  plr::PackedArgs a;
+  a.codes = c->d_codes;
+  a.scales = c->d_scales;
+  a.y = pa.y;
+  a.theta = c->d_theta;
+  a.theta_bias = pa.theta_bias;
+  a.part_g = c->d_part_g;
+  a.part_loss = c->d_part_loss;
+  a.part_res = pa.part_res;
+  a.h_out = pa.h_out;
+  a.z_buf = c->d_z;
+  a.res_in = c->d_res;
+  a.n = c->n;
+  a.row_blocks = c->row_blocks;
+  a.pitch = c->pitch;
+  a.loss_mode = pa.loss_mode;
+  a.identity_link = pa.identity_link;
+  a.z_accumulate = 0;
+  a.kept = 1.;
+  a.mask = plr_mx::Mask{0, 0, 0, 0, 0};
+  const bool drop = grad && c->drop_on;
+  if (drop) {
+    const unsigned t = (unsigned)rint(c->drop.rate * 65536.);
+    a.kept = 65536. / (65536. - t);
+    a.mask = plr_mx::Mask{t, (unsigned)c->drop.seed, (unsigned)(c->drop.seed >> 32),
+                          c->drop.step + (unsigned)std::max(train_round, 0), c->drop.row0};
+  }
+  auto launch = [&](packed_fn f, int blk0, int blocks, int threads) {
+    a.blk0 = blk0;
+    a.blocks = blocks;
+    a.slots = threads / blocks;
+    // each row's partials are summed by as many threads as the tile's rows leave to each
+    a.lanes_per_row = 1;
+    while (a.lanes_per_row < 64 && a.lanes_per_row < blocks &&
+           2 * a.lanes_per_row * a.slots * kPR <= threads)
+      a.lanes_per_row *= 2;
+    hipLaunchKernelGGL(f, dim3(c->grid), dim3(threads), packed_lds(threads, blocks), c->stream, a);
+    return hipGetLastError();
+  };
+  if (!c->packed_sweeps) {
+    PLR_HIP(c, launch(grad ? kPackedGrad[drop] : kPackedEval, 0, (int)c->row_blocks, c->packed_threads));
+    *loss_parts = c->grid;
+    return PLR_OK;
+  }
+  for (int64_t b = 0; b < c->row_blocks; b += kPackedPiece) {
+    const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
+    a.z_accumulate = b > 0;
+    PLR_HIP(c, launch(kPackedDot[drop], (int)b, w, c->packed_threads));
+  }
+  hipLaunchKernelGGL(plr::residual_pass, dim3(c->res_grid), dim3(256), 0, c->stream,
+                     (const double*)c->d_z, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
+                     c->d_part_loss, c->n, pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res,
+                     0, 0, (int64_t)0);
+  PLR_HIP(c, hipGetLastError());
+  *loss_parts = c->res_grid;
+  for (int64_t b = 0; grad && b < c->row_blocks; b += kPackedPiece) {
+    const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
+    PLR_HIP(c, launch(kPackedAxpy[drop], (int)b, w, c->packed_threads));
+  }
+  return PLR_OK;
+}
+
 // Enqueue one pass on the context's stream: streaming kernel (between the two
 // timing events) and finishing kernel.  theta must already be in d_theta.
 // `out` receives d values + the loss; train_round >= 0 makes the finishing
@@ -727,8 +880,12 @@ int enqueue_pass(plr_ctx* c, PassKind kind, unsigned loss_mode, double alpha, do
   pa.z_accumulate = 0;
   pa.res_in = nullptr;
 
+  int packed_parts = 0;
   if (c->timing) PLR_HIP(c, hipEventRecord(c->ev0, c->stream));
-  if (c->lane) {
+  if (c->packed) {
+    const int rc = enqueue_packed(c, pa, grad, train_round, &packed_parts);
+    if (rc != PLR_OK) return rc;
+  } else if (c->lane) {
     hipLaunchKernelGGL(c->lane->fn[grad ? 1 : 0], dim3(grid), dim3(threads), 0, c->stream, pa);
     PLR_HIP(c, hipGetLastError());
   } else if (c->pair) {
@@ -844,7 +1001,7 @@ int enqueue_pass(plr_ctx* c, PassKind kind, unsigned loss_mode, double alpha, do
     fa.part_res = pa.part_res;
     fa.theta_bias = c->d_theta + c->bias_slot;
     fa.nparts = team ? c->nteams : grid;  // a team shares one row of partials
-    fa.nparts_loss = (team || team_dot) ? c->res_grid : grid;
+    fa.nparts_loss = c->packed ? packed_parts : (team || team_dot) ? c->res_grid : grid;
     fa.delta_mode = (kind == kPassDelta) ? (train_round >= 0 ? 2 : 1) : 0;
     fa.have_grad = grad ? 1 : 0;
     const int fblocks = grad ? (int)ceil_div(c->dcols, plr::kFinCols) : 1;
@@ -982,6 +1139,14 @@ bool results_arrived(plr_ctx* c) {
   }
 }
 
+// Dropout belongs to the passes over a shard held in 4 bits.
+int check_dropout(plr_ctx* c) {
+  if (c->drop_on && !c->packed)
+    return fail(c, PLR_ERR_UNSUPPORTED,
+                "dropout is set, but the resident shard is one of doubles: call plr_pack_data first");
+  return PLR_OK;
+}
+
 // One synchronous pass: theta in, kernels, results in the mapped host buffer.
 int run_pass(plr_ctx* c, PassKind kind, const double* theta, unsigned loss_mode,
              double alpha, double beta) {
@@ -990,6 +1155,10 @@ int run_pass(plr_ctx* c, PassKind kind, const double* theta, unsigned loss_mode,
   if (loss_mode > plr::kLossSquared) return fail(c, PLR_ERR_INVALID, "unknown loss flag");
   PLR_HIP(c, hipSetDevice(c->device));
   const bool predict = (kind == kPassPredict || kind == kPassPredictLinear);
+  if (kind == kPassGrad || kind == kPassDelta) {
+    const int rc = check_dropout(c);
+    if (rc != PLR_OK) return rc;
+  }
   if (predict && !c->d_h && !c->h_pred && c->n > 0) {
     // Where the predictions go.  A row of kHostPredictCols columns or more
     // streams slowly enough (8 bytes out per >= 1.5 KiB in) for the host link
@@ -997,7 +1166,8 @@ int run_pass(plr_ctx* c, PassKind kind, const double* theta, unsigned loss_mode,
     // no HBM write traffic disturbing the read stream, no copy command
     // afterwards.  Narrower rows produce predictions faster than the link
     // takes them; they go to device memory and are copied out in a pipeline.
-    if (c->pitch >= kHostPredictCols) {
+    // (4-bit rows are 15 times shorter in bytes for the same width.)
+    if (c->pitch >= (c->packed ? kHostPredictColsPacked : kHostPredictCols)) {
       PLR_HIP(c, hipHostMalloc(&c->h_pred, (size_t)c->n * sizeof(double),
                                hipHostMallocMapped | hipHostMallocCoherent));
       PLR_HIP(c, hipHostGetDevicePointer(reinterpret_cast<void**>(&c->h_pred_dev), c->h_pred, 0));
@@ -1095,6 +1265,8 @@ int plr_set_data_chunk(plr_ctx* c, int64_t row0, int64_t nrows, const double* X,
                        int64_t ldx, const double* y) {
   if (!c) return PLR_ERR_INVALID;
   if (!c->have_data) return fail(c, PLR_ERR_NODATA, "call plr_alloc_data first");
+  if (c->packed)
+    return fail(c, PLR_ERR_UNSUPPORTED, "the shard is held in 4 bits: rows can no longer be replaced");
   return upload_rows(c, row0, nrows, X, ldx, y);
 }
 
@@ -1613,6 +1785,90 @@ int plr_set_data_csv(plr_ctx* c, const char* const* text, const int64_t* len, in
   return rc;
 }
 
+// Rows of a shard held in 4 bits as dense rows of d doubles, constant column included.
+static int unpack_rows(plr_ctx* c, int64_t row0, int64_t m, double* dst) {
+  const int skip = c->bias ? 1 : 0;
+  const int rc = plr_mxfp_dequantize(c->device, c->stream, c->d_codes + row0 * c->row_blocks * 16,
+                                     c->row_blocks * 16, c->d_scales + row0 * c->row_blocks,
+                                     c->row_blocks, m, c->dcols, dst + skip, PLR_F64, c->d);
+  if (rc != PLR_OK) return fail(c, rc, plr_last_error(nullptr));
+  if (skip) {
+    hipLaunchKernelGGL(plr::fill_column, dim3((unsigned)std::min<int64_t>(1024, ceil_div(m, 256))),
+                       dim3(256), 0, c->stream, dst, m, c->d, 1.);
+    PLR_HIP(c, hipGetLastError());
+  }
+  return PLR_OK;
+}
+
+int plr_pack_data(plr_ctx* c) {
+  if (!c) return PLR_ERR_INVALID;
+  if (!c->have_data) return fail(c, PLR_ERR_NODATA, "no shard resident: call plr_set_data first");
+  if (c->packed) return PLR_OK;
+  PLR_HIP(c, hipSetDevice(c->device));
+  PLR_HIP(c, hipStreamSynchronize(c->stream));
+  release_upload_staging(c);
+  const int64_t n = c->n, d = c->d, blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
+  DevBuf codes, scales;
+  if (n > 0) {
+    PLR_HIP(c, hipMalloc(&codes.p, (size_t)n * blocks * 16));
+    PLR_HIP(c, hipMalloc(&scales.p, (size_t)n * blocks));
+    // rows as they lie, or, row-tiled ones, block by block through dense rows
+    const int64_t chunk = c->lane ? std::max<int64_t>(1, (int64_t)(256u << 20) / (d * 8)) : n;
+    DevBuf stage;
+    if (c->lane) PLR_HIP(c, hipMalloc(&stage.p, (size_t)std::min(chunk, n) * d * sizeof(double)));
+    for (int64_t r0 = 0; r0 < n; r0 += chunk) {
+      const int64_t m = std::min(chunk, n - r0);
+      const double* src = c->dX;
+      int64_t ld = c->pitch;
+      if (c->lane) {
+        hipLaunchKernelGGL(plr::gather_rows, dim3((unsigned)ceil_div(m * d, 256)), dim3(256), 0,
+                           c->stream, (const double*)c->dX, c->pitch, c->lane->np, r0, m, (int)d,
+                           c->bias ? 1 : 0, static_cast<double*>(stage.p));
+        PLR_HIP(c, hipGetLastError());
+        src = static_cast<const double*>(stage.p) + (c->bias ? 1 : 0);
+        ld = d;
+      }
+      const int rc = plr_mxfp_quantize(c->device, c->stream, src, PLR_F64, m, c->dcols, ld, 0, nullptr,
+                                       static_cast<uint8_t*>(codes.p) + r0 * blocks * 16, blocks * 16,
+                                       static_cast<uint8_t*>(scales.p) + r0 * blocks, blocks);
+      if (rc != PLR_OK) return fail(c, rc, plr_last_error(nullptr));
+    }
+    PLR_HIP(c, hipStreamSynchronize(c->stream));
+  }
+  // from here on the doubles are gone: the shard is the packed one, or none
+  const bool bias = c->bias;
+  const int64_t dcols = c->dcols;
+  double* const y = c->dy;
+  c->dy = nullptr;
+  free_shape(c);
+  c->n = n;
+  c->d = d;
+  c->bias = bias;
+  c->dcols = dcols;
+  c->dy = y;
+  c->packed = true;
+  c->d_codes = static_cast<uint8_t*>(codes.p);
+  c->d_scales = static_cast<uint8_t*>(scales.p);
+  codes.p = scales.p = nullptr;
+  int rc = plan_packed(c, n);
+  c->bias_slot = c->theta_len;
+  if (rc == PLR_OK) rc = alloc_workspace(c);
+  if (rc != PLR_OK) free_shape(c);  // keeps c->err
+  return rc;
+}
+
+int plr_set_dropout(plr_ctx* c, const plr_dropout* drop) {
+  if (!c) return PLR_ERR_INVALID;
+  if (drop) {
+    if (!(drop->rate >= 0. && rint(drop->rate * 65536.) <= 65535.))
+      return fail(c, PLR_ERR_INVALID, "dropout rate must be at least 0 and at most 65535/65536");
+    if (drop->row0 < 0) return fail(c, PLR_ERR_INVALID, "dropout row0 must be >= 0");
+    c->drop = *drop;
+  }
+  c->drop_on = drop != nullptr;
+  return PLR_OK;
+}
+
 int plr_get_data(plr_ctx* c, int64_t row0, int64_t nrows, double* X, int64_t ldx, double* y) {
   if (!c) return PLR_ERR_INVALID;
   if (!c->have_data) return fail(c, PLR_ERR_NODATA, "no shard resident: call plr_set_data first");
@@ -1632,6 +1888,10 @@ int plr_get_data(plr_ctx* c, int64_t row0, int64_t nrows, double* X, int64_t ldx
     PLR_HIP(c, hipMalloc(&stage.p, (size_t)std::min(chunk_rows, nrows) * d * sizeof(double)));
     for (int64_t r0 = 0; r0 < nrows; r0 += chunk_rows) {
       const int64_t m = std::min(chunk_rows, nrows - r0);
+      if (c->packed) {
+        const int rc = unpack_rows(c, row0 + r0, m, static_cast<double*>(stage.p));
+        if (rc != PLR_OK) return rc;
+      } else
       hipLaunchKernelGGL(plr::gather_rows, dim3((unsigned)ceil_div(m * d, 256)), dim3(256), 0,
                          c->stream, (const double*)c->dX, c->pitch, c->lane ? c->lane->np : 0,
                          row0 + r0, m, (int)d, c->bias ? 1 : 0, static_cast<double*>(stage.p));
@@ -1696,6 +1956,8 @@ int plr_train_dgd(plr_ctx* c, double* theta, double alpha, double beta, int roun
   if (!c) return PLR_ERR_INVALID;
   if (!c->have_data) return fail(c, PLR_ERR_NODATA, "no shard resident: call plr_set_data first");
   if (!theta || rounds < 0) return fail(c, PLR_ERR_INVALID, "need theta and rounds >= 0");
+  int rc = check_dropout(c);
+  if (rc != PLR_OK) return rc;
   if (rounds == 0) return PLR_OK;
   PLR_HIP(c, hipSetDevice(c->device));
   if (c->curve_len < rounds) {
@@ -1708,7 +1970,6 @@ int plr_train_dgd(plr_ctx* c, double* theta, double alpha, double beta, int roun
     PLR_HIP(c, hipMalloc(&c->d_train_out, (size_t)(c->d + 1) * sizeof(double)));
   const unsigned loss_mode = loss_curve ? plr::kLossReference : plr::kLossNone;
   const int skip = c->bias ? 1 : 0;
-  int rc = PLR_OK;
   for (int attempt = 0;; ++attempt) {
     rc = stage_theta_from_host(c, theta);
     if (rc != PLR_OK) return rc;
@@ -2067,17 +2328,20 @@ int plr_probe_read_bandwidth(plr_ctx* c, int reps, double* gb_per_s) {
   if (!gb_per_s || reps < 1) return fail(c, PLR_ERR_INVALID, "need reps >= 1 and an output");
   if (!c->have_data || c->n == 0) return fail(c, PLR_ERR_NODATA, "no shard resident");
   PLR_HIP(c, hipSetDevice(c->device));
-  const size_t bytes = (size_t)c->n * c->pitch * sizeof(double);
+  const size_t bytes = c->packed ? (size_t)c->n * c->row_blocks * 16
+                                 : (size_t)c->n * c->pitch * sizeof(double);
+  const void* const base = c->packed ? static_cast<const void*>(c->d_codes)
+                                    : static_cast<const void*>(c->dX);
   const int64_t ntiles = (int64_t)(bytes / 8192);
   if (ntiles < 1) return fail(c, PLR_ERR_INVALID, "shard smaller than one 8 KiB tile");
   const int grid = c->num_cu;
   for (int i = 0; i < 2; ++i)
     hipLaunchKernelGGL(plr::read_probe, dim3(grid), dim3(256), 0, c->stream,
-                       reinterpret_cast<const plr::v2d*>(c->dX), ntiles, c->d_part_loss);
+                       static_cast<const plr::v2d*>(base), ntiles, c->d_part_loss);
   PLR_HIP(c, hipEventRecord(c->ev0, c->stream));
   for (int i = 0; i < reps; ++i)
     hipLaunchKernelGGL(plr::read_probe, dim3(grid), dim3(256), 0, c->stream,
-                       reinterpret_cast<const plr::v2d*>(c->dX), ntiles, c->d_part_loss);
+                       static_cast<const plr::v2d*>(base), ntiles, c->d_part_loss);
   PLR_HIP(c, hipGetLastError());
   PLR_HIP(c, hipEventRecord(c->ev1, c->stream));
   PLR_HIP(c, hipStreamSynchronize(c->stream));

@@ -1566,6 +1566,13 @@ __global__ __launch_bounds__(256) void stage_theta_padded(const double* __restri
     dst[i] = i < d ? src[i] : 0.;
 }
 
+// Column 0 of m rows at a pitch of ld doubles set to v.
+__global__ __launch_bounds__(256) void fill_column(double* dst, int64_t m, int64_t ld, double v) {
+  for (int64_t i = threadIdx.x + (int64_t)blockIdx.x * blockDim.x; i < m;
+       i += (int64_t)gridDim.x * blockDim.x)
+    dst[i * ld] = v;
+}
+
 // Plain fill with zeros (a kernel, not a memset command: safe inside a
 // captured graph).
 __global__ __launch_bounds__(256) void fill_zero(double* __restrict__ dst, int64_t count) {

@@ -1,0 +1,691 @@
+// Operators on device matrices: quantisation to microscaled 4-bit floating point and back, the
+// product of two such matrices, and dropout.  The entry points (include/plr.h) take device
+// pointers and a stream, enqueue kernels and return; they allocate nothing and keep nothing
+// between calls.
+#include "../../include/plr.h"
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "plr_internal.hpp"
+#include "plr_matmul.hpp"
+#include "plr_mxfp.hpp"
+
+namespace {
+
+using namespace plr_mx;
+
+// ---------------------------------------------------------------- element types
+template <typename T>
+struct Elem;
+template <>
+struct Elem<double> {
+  typedef double wide;  // what a value is worked on in
+  static __device__ __forceinline__ double up(double v) { return v; }
+  static __device__ __forceinline__ double down(double v) { return v; }
+};
+template <>
+struct Elem<float> {
+  typedef float wide;
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <>
+struct Elem<__bf16> {
+  typedef float wide;
+  static __device__ __forceinline__ float up(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 down(float v) { return (__bf16)v; }
+};
+template <>
+struct Elem<_Float16> {
+  typedef float wide;
+  static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
+};
+
+// V consecutive values, moved as 16-byte words where the caller knows them aligned.
+template <typename T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+  T v[V];
+};
+
+// Columns c .. c + V of a row at p (p = the row's first value); those at `cols` and behind are 0.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p, int64_t c, int64_t cols, bool whole) {
+  Pack<T, V> r;
+  if (whole && c + V <= cols) {
+    r = *reinterpret_cast<const Pack<T, V>*>(p + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = c + i < cols ? p[c + i] : T(0);
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, int64_t c, int64_t cols, bool whole,
+                                           const Pack<T, V>& r) {
+  if (whole && c + V <= cols) {
+    *reinterpret_cast<Pack<T, V>*>(p + c) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < cols) p[c + i] = r.v[i];
+  }
+}
+
+// ---------------------------------------------------------------- quantisation
+// The bits of |v| that order magnitudes and hold the exponent: for doubles the high word.
+__device__ __forceinline__ unsigned mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned mag_bits(double v) {
+  return (unsigned)__double2hiint(v) & 0x7fffffffu;
+}
+// Scale byte of a block from the largest mag_bits: floor(log2 max) - 2 (6 = 1.5 * 2^2 is the
+// largest code), biased by 127, at least 0; 255 when a value is not finite.  NaN and infinity
+// order above every finite value, so one maximum finds them too.
+__device__ __forceinline__ unsigned scale_byte(unsigned top, float) {
+  const unsigned e = top >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+__device__ __forceinline__ unsigned scale_byte(unsigned top, double) {
+  const int e = (int)(top >> 20);
+  if (e == 2047) return 255u;
+  const int s = e - 1023 - 2 + 127;
+  return (unsigned)(s < 0 ? 0 : s > 254 ? 254 : s);
+}
+
+// Eight values to eight codes, nearest with ties to the even code, saturating at 6.
+__device__ __forceinline__ unsigned encode8(const float (&v)[8], unsigned s) {
+  const float sc = scale_value(s);
+  unsigned w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], sc, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], sc, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], sc, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], sc, 3);
+  return w;
+}
+// Doubles are scaled, then cut to a float's 24 bits with a last bit that says whether anything
+// was cut off: the one rounding to four bits then goes the way the double's own would (a plain
+// conversion to float could land on a tie the double is not on).
+__device__ __forceinline__ float sticky_float(double v) {
+  const int hi = __double2hiint(v);
+  unsigned lo = (unsigned)__double2loint(v);
+  lo = (lo & 0xe0000000u) | ((lo & 0x1fffffffu) ? 0x20000000u : 0u);
+  return (float)__hiloint2double(hi, (int)lo);
+}
+__device__ __forceinline__ unsigned encode8(const double (&v)[8], unsigned s) {
+  // 2^-(s - 127); doubles far outside a float's range meet s = 254 or s = 0 and saturate or vanish
+  const double inv = __hiloint2double((int)((1023u + 127u - s) << 20), 0);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = sticky_float(fmin(fmax(v[i] * inv, -8.), 8.));
+  return encode8(f, 127u);
+}
+
+struct QuantArgs {
+  const void* x;
+  int64_t n, d, ldx;
+  uint8_t* codes;
+  int64_t ldc;
+  uint8_t* scales;
+  int64_t lds;
+  int64_t chunks;  // 128-column chunks of an output row that are written
+  int wide_load;   // rows of x start on 16-byte boundaries
+  int tc_log2;     // a workgroup's tile is 2^tc_log2 chunks wide
+  unsigned nbx;    // tiles across
+  Mask mask;
+};
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantRows = 4;  // row sets per workgroup: as many loads in flight per thread
+
+// Largest of the four lanes of a quad, in all four.
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+  unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);  // lanes 1 0 3 2
+  v = v > o ? v : o;
+  o = (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);  // lanes 2 3 0 1
+  return v > o ? v : o;
+}
+
+// Blocks along a row.  A thread takes 8 columns, a quad a block, 16 lanes a chunk of 128 columns;
+// the workgroup's 16 chunk slots are 2^tc across and 16 / 2^tc rows.  Bound by the bytes of x.
+template <typename T, bool DROP>
+__global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
+  typedef typename Elem<T>::wide W;
+  const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
+  const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
+  const int rows = 16 >> a.tc_log2;  // rows per set
+  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8;
+  const T* x = static_cast<const T*>(a.x);
+  Pack<T, 8> in[kQuantRows];
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r < a.n) in[u] = load_pack<T, 8>(x + r * a.ldx, c, a.d, a.wide_load);
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r >= a.n) continue;  // (a quad shares its row: its lanes leave together)
+    W v[8];
+    unsigned top = 0;
+    const unsigned keep = DROP ? keep8(a.mask, r, (unsigned)(c >> 3)) : 0xffu;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = Elem<T>::up(in[u].v[i]);
+      if (DROP && !(keep >> i & 1)) v[i] = W(0);
+      const unsigned b = mag_bits(v[i]);
+      top = b > top ? b : top;
+    }
+    top = quad_max(top);
+    const unsigned s = scale_byte(top, W(0));
+    const unsigned w = s == 255u ? 0u : encode8(v, s);
+    if (c / 2 < a.ldc && chunk < a.chunks)
+      *reinterpret_cast<unsigned*>(a.codes + r * a.ldc + c / 2) = w;
+    if ((l16 & 3) == 0 && c / 32 < a.lds && chunk < a.chunks)
+      a.scales[r * a.lds + c / 32] = (uint8_t)s;
+  }
+}
+
+// Blocks along a column: row j of the result is column j of x.  A thread holds V = 16 bytes of
+// columns times 32 rows in registers -- so a block never leaves its thread --, 8 lanes cover 128
+// bytes of a row of x and the 8 groups of lanes 256 rows, so that a result row is written in
+// pieces of 128 bytes.
+template <typename T, bool DROP>
+__global__ __launch_bounds__(64) void quantize_columns(QuantArgs a) {
+  typedef typename Elem<T>::wide W;
+  constexpr int V = 16 / (int)sizeof(T);
+  const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
+  const int lane = threadIdx.x;
+  const int64_t c0 = ((int64_t)bx * 8 + (lane & 7)) * V;  // first column of x
+  const int64_t blk = (int64_t)by * 8 + (lane >> 3);      // block of 32 rows
+  const int64_t r0 = blk * 32;
+  if (c0 >= a.d || blk * 16 >= a.ldc || blk >= a.chunks * 4) return;
+  const T* x = static_cast<const T*>(a.x);
+  Pack<T, V> in[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (r0 + i < a.n) {
+      in[i] = load_pack<T, V>(x + (r0 + i) * a.ldx, c0, a.d, a.wide_load);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) in[i].v[k] = T(0);
+    }
+  }
+  if (DROP) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const unsigned keep = keep8(a.mask, r0 + i, (unsigned)(c0 >> 3)) >> (c0 & 7);
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (!(keep >> k & 1)) in[i].v[k] = T(0);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    if (c0 + k >= a.d) break;
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const unsigned b = mag_bits(Elem<T>::up(in[i].v[k]));
+      top = b > top ? b : top;
+    }
+    const unsigned s = scale_byte(top, W(0));
+    uint4 w;
+    unsigned* ww = reinterpret_cast<unsigned*>(&w);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      W v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = Elem<T>::up(in[8 * q + i].v[k]);
+      ww[q] = s == 255u ? 0u : encode8(v, s);
+    }
+    *reinterpret_cast<uint4*>(a.codes + (c0 + k) * a.ldc + blk * 16) = w;
+    if (blk < a.lds) a.scales[(c0 + k) * a.lds + blk] = (uint8_t)s;
+  }
+}
+
+struct DequantArgs {
+  const uint8_t* codes;
+  int64_t ldc;
+  const uint8_t* scales;
+  int64_t lds;
+  void* out;
+  int64_t n, d, ldo;
+  int wide_store;
+  int tc_log2;
+  unsigned nbx;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) {
+  typedef typename Elem<T>::wide W;
+  const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
+  const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
+  const int rows = 16 >> a.tc_log2;
+  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8;
+  if (c >= a.d) return;
+  unsigned w[kQuantRows], s[kQuantRows];
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r < a.n) {
+      w[u] = *reinterpret_cast<const unsigned*>(a.codes + r * a.ldc + c / 2);
+      s[u] = a.scales[r * a.lds + c / 32];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r >= a.n) continue;
+    // the product with the scale is exact in the wide type unless it leaves its range
+    const v2f q[4] = {decode2<0>(w[u]), decode2<1>(w[u]), decode2<2>(w[u]), decode2<3>(w[u])};
+    const W sc = s[u] == 255u ? W(__builtin_nanf("")) : sizeof(W) == 8 ? W(scale_value_f64(s[u]))
+                                                                       : W(scale_value(s[u]));
+    Pack<T, 8> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = Elem<T>::down((W)q[i >> 1][i & 1] * sc);
+    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
+  }
+}
+
+// ---------------------------------------------------------------- dropout
+struct DropArgs {
+  const void* x;
+  void* out;
+  int64_t n, d, ldx, ldo;
+  int wide_load, wide_store;
+  int tc_log2;
+  unsigned nbx;
+  double scale;
+  Mask mask;
+};
+
+// A thread takes 8 columns, one generator call; bound by the bytes moved.
+template <typename T>
+__global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
+  typedef typename Elem<T>::wide W;
+  const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
+  const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+  const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
+  const int rows = 16 >> a.tc_log2;
+  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8;
+  if (c >= a.d) return;
+  Pack<T, 8> in[kQuantRows];
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r < a.n) in[u] = load_pack<T, 8>(static_cast<const T*>(a.x) + r * a.ldx, c, a.d, a.wide_load);
+  }
+  const W sc = (W)a.scale;
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = row + (int64_t)u * rows;
+    if (r >= a.n) continue;
+    const unsigned keep = keep8(a.mask, r, (unsigned)(c >> 3));
+    Pack<T, 8> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      o.v[i] = (keep >> i & 1) ? Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc) : T(0);
+    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int kMaxDevices = 64;
+std::atomic<int> g_cu[kMaxDevices];  // compute units of a checked gfx950 device, 0: not looked at
+
+int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
+
+// One call: the caller's current device is left as it was found, failures are recorded under the
+// entry point's name.
+struct Call {
+  const char* name;
+  int prev = -1;
+  hipStream_t stream = nullptr;
+  int cus = 0;
+  explicit Call(const char* entry) : name(entry) {}
+  ~Call() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+  int bad(int code, const char* what) const {
+    char b[256];
+    snprintf(b, sizeof b, "%s: %s", name, what);
+    return plr_fail_without_context(code, b);
+  }
+  int hip(hipError_t e, const char* what) const {
+    char b[256];
+    (void)hipGetLastError();
+    snprintf(b, sizeof b, "%s: %s failed: %s", name, what, hipGetErrorString(e));
+    return plr_fail_without_context(e == hipErrorOutOfMemory ? PLR_ERR_NOMEM : PLR_ERR_HIP, b);
+  }
+  int begin(int device_id, void* hip_stream) {
+    stream = reinterpret_cast<hipStream_t>(hip_stream);
+    if (device_id < 0 || device_id >= kMaxDevices)
+      return bad(PLR_ERR_INVALID, "device_id out of range");
+    int cur = -1;
+    hipError_t e = hipGetDevice(&cur);
+    if (e != hipSuccess) return hip(e, "hipGetDevice");
+    if (cur != device_id) {
+      if ((e = hipSetDevice(device_id)) != hipSuccess) return hip(e, "hipSetDevice");
+      prev = cur;
+    }
+    cus = g_cu[device_id].load();
+    if (cus == 0) {
+      // once per device; not stream work, so a caller that captures makes one call before
+      hipDeviceProp_t prop;
+      if ((e = hipGetDeviceProperties(&prop, device_id)) != hipSuccess)
+        return hip(e, "hipGetDeviceProperties");
+      if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
+        return bad(PLR_ERR_UNSUPPORTED, "this library carries gfx950 code only");
+      cus = prop.multiProcessorCount;
+      g_cu[device_id].store(cus);
+    }
+    return PLR_OK;
+  }
+  int launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? (int)PLR_OK : hip(e, "launch");
+  }
+};
+
+size_t type_size(unsigned t) {
+  switch (t) {
+    case PLR_F64: return 8;
+    case PLR_F32: return 4;
+    case PLR_BF16:
+    case PLR_F16: return 2;
+  }
+  return 0;
+}
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// rows * pitch elements of `size` bytes can be addressed
+bool fits(int64_t rows, int64_t pitch, size_t size) {
+  return rows == 0 || pitch <= INT64_MAX / (int64_t)size / rows;
+}
+
+int check_mask(Call& c, const plr_dropout* drop, Mask* m, double* scale) {
+  *m = Mask{0, 0, 0, 0, 0};
+  *scale = 1.;
+  if (!drop) return PLR_OK;
+  if (!(drop->rate >= 0. && drop->rate < 1.))
+    return c.bad(PLR_ERR_INVALID, "dropout rate must be at least 0 and below 1");
+  const unsigned t = (unsigned)rint(drop->rate * 65536.);
+  if (t > 65535u)
+    return c.bad(PLR_ERR_INVALID, "dropout rate must be at most 65535/65536");
+  if (drop->row0 < 0) return c.bad(PLR_ERR_INVALID, "dropout row0 must be >= 0");
+  m->threshold = t;
+  m->key0 = (unsigned)drop->seed;
+  m->key1 = (unsigned)(drop->seed >> 32);
+  m->step = drop->step;
+  m->row0 = drop->row0;
+  *scale = 65536. / (65536. - t);
+  return PLR_OK;
+}
+
+// Tiles of 16 chunk slots: as wide as the row needs, at most 16 chunks.
+int tile_log2(int64_t chunks) {
+  int t = 0;
+  while (t < 4 && (int64_t)(1 << t) < chunks) ++t;
+  return t;
+}
+
+// A launch counts its threads in 32 bits.
+bool fits_launch(int64_t x, int64_t y, int threads) {
+  return y == 0 || x <= (int64_t)0xffffffffu / threads / y;
+}
+
+// Workgroups of the tiled kernels; false when a launch cannot hold them.
+bool tile_grid(int64_t n, int64_t chunks, int tc, unsigned* nbx, unsigned* grid) {
+  const int64_t x = ceil_div(chunks, (int64_t)1 << tc);
+  const int64_t y = ceil_div(n, (int64_t)(16 >> tc) * kQuantRows);
+  if (!fits_launch(x, y, kQuantThreads)) return false;
+  *nbx = (unsigned)x;
+  *grid = (unsigned)(x * y);
+  return true;
+}
+
+template <typename T>
+void launch_quantize(const QuantArgs& a, bool transpose, bool drop, unsigned grid, hipStream_t st) {
+  if (transpose) {
+    auto f = drop ? quantize_columns<T, true> : quantize_columns<T, false>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(64), 0, st, a);
+  } else {
+    auto f = drop ? quantize_rows<T, true> : quantize_rows<T, false>;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(kQuantThreads), 0, st, a);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t plr_mxfp_code_pitch(int64_t d) { return d < 1 || d > INT64_MAX - 128 ? 0 : ceil_div(d, 128) * 64; }
+int64_t plr_mxfp_scale_pitch(int64_t d) { return d < 1 || d > INT64_MAX - 128 ? 0 : ceil_div(d, 128) * 4; }
+
+int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned type, int64_t n,
+                      int64_t d, int64_t ldx, unsigned flags, const plr_dropout* drop,
+                      uint8_t* dcodes, int64_t ldc, uint8_t* dscales, int64_t lds) {
+  Call c("plr_mxfp_quantize");
+  const size_t size = type_size(type);
+  if (size == 0) return c.bad(PLR_ERR_INVALID, "unknown element type");
+  if (flags & ~(unsigned)PLR_MXFP_TRANSPOSE) return c.bad(PLR_ERR_INVALID, "unknown flag");
+  if (n < 0 || d < 1) return c.bad(PLR_ERR_INVALID, "need n >= 0 and d >= 1");
+  if (ldx < d) return c.bad(PLR_ERR_INVALID, "ldx must be >= d");
+  const bool tr = (flags & PLR_MXFP_TRANSPOSE) != 0;
+  const int64_t rows = tr ? d : n, cols = tr ? n : d;  // of the result
+  if (d > (int64_t)1 << 34 || (tr && n > (int64_t)1 << 34))
+    return c.bad(PLR_ERR_INVALID, "a row of more than 2^34 values");
+  const int64_t blocks = ceil_div(cols, kBlockCols);
+  if (ldc % 16 != 0 || ldc < blocks * 16)
+    return c.bad(PLR_ERR_INVALID, "code pitch must be a multiple of 16 and hold the row's blocks of 16 bytes");
+  if (lds < blocks) return c.bad(PLR_ERR_INVALID, "scale pitch must hold a byte per block of 32 columns");
+  if (!fits(n, ldx, size) || !fits(rows, ldc, 1) || !fits(rows, lds, 1))
+    return c.bad(PLR_ERR_INVALID, "matrix too large to address");
+  Mask mask;
+  double scale;
+  int rc = check_mask(c, drop, &mask, &scale);
+  if (rc != PLR_OK) return rc;
+  if (n > 0 && (!dx || !dcodes || !dscales))
+    return c.bad(PLR_ERR_INVALID, "device pointers must not be NULL");
+  if (!aligned(dx, size)) return c.bad(PLR_ERR_INVALID, "dx must be aligned to its element type");
+  if (!aligned(dcodes, 16)) return c.bad(PLR_ERR_INVALID, "dcodes must be 16-byte aligned");
+  QuantArgs a;
+  a.x = dx;
+  a.n = n;
+  a.d = d;
+  a.ldx = ldx;
+  a.codes = dcodes;
+  a.ldc = ldc;
+  a.scales = dscales;
+  a.lds = lds;
+  // whole 128-column chunks are written as far as the pitches reach
+  a.chunks = ceil_div(cols, 128);
+  a.wide_load = aligned(dx, 16) && ldx * (int64_t)size % 16 == 0;
+  a.mask = mask;
+  a.tc_log2 = 0;
+  unsigned grid = 0;
+  if (tr) {
+    const int64_t x = ceil_div(d, 8 * (16 / (int64_t)size)), y = ceil_div(a.chunks * 4, 8);
+    if (!fits_launch(x, y, 64)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+    a.nbx = (unsigned)x;
+    grid = (unsigned)(x * y);
+  } else {
+    a.tc_log2 = tile_log2(a.chunks);
+    if (!tile_grid(n, a.chunks, a.tc_log2, &a.nbx, &grid))
+      return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+  }
+  rc = c.begin(device_id, hip_stream);
+  if (rc != PLR_OK || n == 0) return rc;
+  const bool dr = drop != nullptr && mask.threshold > 0;
+  switch (type) {
+    case PLR_F64: launch_quantize<double>(a, tr, dr, grid, c.stream); break;
+    case PLR_F32: launch_quantize<float>(a, tr, dr, grid, c.stream); break;
+    case PLR_BF16: launch_quantize<__bf16>(a, tr, dr, grid, c.stream); break;
+    default: launch_quantize<_Float16>(a, tr, dr, grid, c.stream); break;
+  }
+  return c.launched();
+}
+
+int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, int64_t ldc,
+                        const uint8_t* dscales, int64_t lds, int64_t n, int64_t d, void* dout,
+                        unsigned type, int64_t ldo) {
+  Call c("plr_mxfp_dequantize");
+  const size_t size = type_size(type);
+  if (size == 0) return c.bad(PLR_ERR_INVALID, "unknown element type");
+  if (n < 0 || d < 1) return c.bad(PLR_ERR_INVALID, "need n >= 0 and d >= 1");
+  if (d > (int64_t)1 << 34) return c.bad(PLR_ERR_INVALID, "a row of more than 2^34 values");
+  if (ldo < d) return c.bad(PLR_ERR_INVALID, "ldo must be >= d");
+  const int64_t blocks = ceil_div(d, kBlockCols);
+  if (ldc % 16 != 0 || ldc < blocks * 16)
+    return c.bad(PLR_ERR_INVALID, "code pitch must be a multiple of 16 and hold the row's blocks of 16 bytes");
+  if (lds < blocks) return c.bad(PLR_ERR_INVALID, "scale pitch must hold a byte per block of 32 columns");
+  if (!fits(n, ldo, size) || !fits(n, ldc, 1) || !fits(n, lds, 1))
+    return c.bad(PLR_ERR_INVALID, "matrix too large to address");
+  if (n > 0 && (!dout || !dcodes || !dscales))
+    return c.bad(PLR_ERR_INVALID, "device pointers must not be NULL");
+  if (!aligned(dout, size)) return c.bad(PLR_ERR_INVALID, "dout must be aligned to its element type");
+  if (!aligned(dcodes, 16)) return c.bad(PLR_ERR_INVALID, "dcodes must be 16-byte aligned");
+  DequantArgs a;
+  a.codes = dcodes;
+  a.ldc = ldc;
+  a.scales = dscales;
+  a.lds = lds;
+  a.out = dout;
+  a.n = n;
+  a.d = d;
+  a.ldo = ldo;
+  a.wide_store = aligned(dout, 16) && ldo * (int64_t)size % 16 == 0;
+  const int64_t chunks = ceil_div(d, 128);
+  a.tc_log2 = tile_log2(chunks);
+  unsigned grid = 0;
+  if (!tile_grid(n, chunks, a.tc_log2, &a.nbx, &grid))
+    return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+  int rc = c.begin(device_id, hip_stream);
+  if (rc != PLR_OK || n == 0) return rc;
+  const dim3 g(grid), t(kQuantThreads);
+  switch (type) {
+    case PLR_F64: hipLaunchKernelGGL(dequantize_rows<double>, g, t, 0, c.stream, a); break;
+    case PLR_F32: hipLaunchKernelGGL(dequantize_rows<float>, g, t, 0, c.stream, a); break;
+    case PLR_BF16: hipLaunchKernelGGL(dequantize_rows<__bf16>, g, t, 0, c.stream, a); break;
+    default: hipLaunchKernelGGL(dequantize_rows<_Float16>, g, t, 0, c.stream, a); break;
+  }
+  return c.launched();
+}
+
+int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned type, int64_t n,
+                      int64_t d, int64_t ldx, void* dout, int64_t ldo, const plr_dropout* drop) {
+  Call c("plr_dropout_apply");
+  const size_t size = type_size(type);
+  if (size == 0) return c.bad(PLR_ERR_INVALID, "unknown element type");
+  if (n < 0 || d < 1) return c.bad(PLR_ERR_INVALID, "need n >= 0 and d >= 1");
+  if (d > (int64_t)1 << 34) return c.bad(PLR_ERR_INVALID, "a row of more than 2^34 values");
+  if (ldx < d || ldo < d) return c.bad(PLR_ERR_INVALID, "ldx and ldo must be >= d");
+  if (!fits(n, ldx, size) || !fits(n, ldo, size))
+    return c.bad(PLR_ERR_INVALID, "matrix too large to address");
+  if (!drop) return c.bad(PLR_ERR_INVALID, "drop must not be NULL");
+  DropArgs a;
+  int rc = check_mask(c, drop, &a.mask, &a.scale);
+  if (rc != PLR_OK) return rc;
+  if (n > 0 && (!dx || !dout)) return c.bad(PLR_ERR_INVALID, "device pointers must not be NULL");
+  if (!aligned(dx, size) || !aligned(dout, size))
+    return c.bad(PLR_ERR_INVALID, "dx and dout must be aligned to their element type");
+  a.x = dx;
+  a.out = dout;
+  a.n = n;
+  a.d = d;
+  a.ldx = ldx;
+  a.ldo = ldo;
+  a.wide_load = aligned(dx, 16) && ldx * (int64_t)size % 16 == 0;
+  a.wide_store = aligned(dout, 16) && ldo * (int64_t)size % 16 == 0;
+  const int64_t chunks = ceil_div(d, 128);
+  a.tc_log2 = tile_log2(chunks);
+  unsigned grid = 0;
+  if (!tile_grid(n, chunks, a.tc_log2, &a.nbx, &grid))
+    return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+  rc = c.begin(device_id, hip_stream);
+  if (rc != PLR_OK || n == 0) return rc;
+  const dim3 g(grid), t(kQuantThreads);
+  switch (type) {
+    case PLR_F64: hipLaunchKernelGGL(dropout_rows<double>, g, t, 0, c.stream, a); break;
+    case PLR_F32: hipLaunchKernelGGL(dropout_rows<float>, g, t, 0, c.stream, a); break;
+    case PLR_BF16: hipLaunchKernelGGL(dropout_rows<__bf16>, g, t, 0, c.stream, a); break;
+    default: hipLaunchKernelGGL(dropout_rows<_Float16>, g, t, 0, c.stream, a); break;
+  }
+  return c.launched();
+}
+
+int64_t plr_mxfp_matmul_workspace(int64_t m, int64_t n, int64_t k) {
+  (void)m;
+  (void)n;
+  (void)k;
+  return 0;
+}
+
+int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64_t k,
+                    const uint8_t* da, int64_t lda, const uint8_t* dsa, int64_t ldsa,
+                    const uint8_t* db, int64_t ldb, const uint8_t* dsb, int64_t ldsb, double alpha,
+                    const plr_dropout* drop, void* dc, unsigned type, int64_t ldc, void* workspace,
+                    int64_t workspace_bytes) {
+  Call c("plr_mxfp_matmul");
+  const size_t size = type_size(type);
+  if (size == 0 || type == PLR_F64)
+    return c.bad(PLR_ERR_INVALID, "the result is PLR_F32, PLR_BF16 or PLR_F16");
+  if (m < 0 || n < 0 || k < 1) return c.bad(PLR_ERR_INVALID, "need m >= 0, n >= 0 and k >= 1");
+  if (m > (int64_t)1 << 31 || n > (int64_t)1 << 31 || k > (int64_t)1 << 31)
+    return c.bad(PLR_ERR_INVALID, "m, n and k must be at most 2^31");
+  if (lda % 64 != 0 || ldb % 64 != 0 || lda < plr_mxfp_code_pitch(k) || ldb < plr_mxfp_code_pitch(k))
+    return c.bad(PLR_ERR_INVALID, "code pitches must be multiples of 64 and at least plr_mxfp_code_pitch(k)");
+  if (ldsa % 4 != 0 || ldsb % 4 != 0 || ldsa < plr_mxfp_scale_pitch(k) || ldsb < plr_mxfp_scale_pitch(k))
+    return c.bad(PLR_ERR_INVALID, "scale pitches must be multiples of 4 and at least plr_mxfp_scale_pitch(k)");
+  if (ldc < n) return c.bad(PLR_ERR_INVALID, "ldc must be >= n");
+  if (!fits(m, lda, 1) || !fits(n, ldb, 1) || !fits(m, ldsa, 1) || !fits(n, ldsb, 1) || !fits(m, ldc, size))
+    return c.bad(PLR_ERR_INVALID, "matrix too large to address");
+  MatmulArgs a;
+  double scale;
+  int rc = check_mask(c, drop, &a.mask, &scale);
+  if (rc != PLR_OK) return rc;
+  const int64_t need = plr_mxfp_matmul_workspace(m, n, k);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return c.bad(PLR_ERR_INVALID, "workspace smaller than plr_mxfp_matmul_workspace(m, n, k)");
+  if (m > 0 && n > 0) {
+    if (!da || !dsa || !db || !dsb || !dc)
+      return c.bad(PLR_ERR_INVALID, "device pointers must not be NULL");
+    if (!aligned(da, 16) || !aligned(db, 16)) return c.bad(PLR_ERR_INVALID, "da and db must be 16-byte aligned");
+    if (!aligned(dsa, 4) || !aligned(dsb, 4)) return c.bad(PLR_ERR_INVALID, "dsa and dsb must be 4-byte aligned");
+    if (!aligned(dc, size)) return c.bad(PLR_ERR_INVALID, "dc must be aligned to its element type");
+  }
+  a.a = da;
+  a.b = db;
+  a.sa = dsa;
+  a.sb = dsb;
+  a.lda = lda;
+  a.ldb = ldb;
+  a.ldsa = ldsa;
+  a.ldsb = ldsb;
+  a.m = m;
+  a.n = n;
+  a.chunks = (int)ceil_div(k, 128);
+  a.c = dc;
+  a.ldc = ldc;
+  a.alpha = (float)alpha;
+  a.kept = (float)scale;
+  rc = c.begin(device_id, hip_stream);
+  if (rc != PLR_OK || m == 0 || n == 0) return rc;
+  const bool dr = drop != nullptr && a.mask.threshold > 0;
+  if (!launch_matmul(a, type == PLR_F32 ? 0 : type == PLR_BF16 ? 1 : 2, dr, c.cus, c.stream))
+    return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+  return c.launched();
+}
+
+}  // extern "C"
