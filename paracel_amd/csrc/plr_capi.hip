@@ -213,18 +213,29 @@ int g_na_num_cu[kNaMaxDevices] = {};
 int g_na_occ[kNaMaxDevices][kNaMaxPitch / plr::kChunkCols + 1] = {};
 std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 
-// Shard held in 4 bits: kernel instances [dropout].  A row of up to kPackedFused blocks is read
-// once; wider ones go in column pieces of kPackedPiece blocks, in two sweeps.
+// Shard held in 4 bits.  A row of up to kPackedFused blocks is read once (theta and the partial
+// dot products of two tiles have to fit a compute unit's LDS); wider ones go in column pieces of
+// kPackedPiece blocks, in two sweeps.
 typedef void (*packed_fn)(plr::PackedArgs);
+struct PackedFns {
+  int stride;         // blocks of theta in LDS: the widest row
+  packed_fn grad[2];  // [dropout]
+  packed_fn eval;
+};
+template <int STRIDE>
+constexpr PackedFns make_packed() {
+  return {STRIDE,
+          {plr::packed_pass<true, false, plr::kPassFused, STRIDE>,
+           plr::packed_pass<true, true, plr::kPassFused, STRIDE>},
+          plr::packed_pass<false, false, plr::kPassFused, STRIDE>};
+}
+const PackedFns kPacked[3] = {make_packed<64>(), make_packed<256>(), make_packed<512>()};
+const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, 256>,
+                                 plr::packed_pass<false, true, plr::kPassDot, 256>};
+const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, 256>,
+                                  plr::packed_pass<true, true, plr::kPassAxpy, 256>};
 constexpr int kPR = plr::kPackedRows;
-const packed_fn kPackedGrad[2] = {plr::packed_pass<true, false, plr::kPassFused, kPR>,
-                                  plr::packed_pass<true, true, plr::kPassFused, kPR>};
-const packed_fn kPackedEval = plr::packed_pass<false, false, plr::kPassFused, kPR>;
-const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, kPR>,
-                                 plr::packed_pass<false, true, plr::kPassDot, kPR>};
-const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, kPR>,
-                                  plr::packed_pass<true, true, plr::kPassAxpy, kPR>};
-constexpr int kPackedFused = 512, kPackedPiece = 256;
+constexpr int kPackedFused = 480, kPackedPiece = 256;
 
 }  // namespace
 
@@ -331,6 +342,7 @@ struct plr_ctx {
   uint8_t* d_codes = nullptr;     // n x row_blocks * 16 bytes
   uint8_t* d_scales = nullptr;    // n x row_blocks
   int64_t row_blocks = 0;
+  const PackedFns* packed_fns = nullptr;
   int packed_threads = 0;
   bool packed_sweeps = false;     // too wide for one read: column pieces, two sweeps
   bool drop_on = false;           // plr_set_dropout
@@ -594,15 +606,18 @@ int plan_shape(plr_ctx* c, int64_t n, int64_t d) {
   return PLR_OK;
 }
 
-// Threads of a workgroup for pieces of `blocks` blocks: 256 or 512, whichever leaves fewer idle.
+// Threads of a workgroup for rows of `blocks` blocks: two workgroups of 256 per compute unit or
+// one of 512, whichever leaves fewer threads idle.
 int packed_workgroup(int blocks) {
-  if (blocks > 256) return 512;
+  if (blocks > 64) return 512;
   return (512 / blocks) > 2 * (256 / blocks) ? 512 : 256;
 }
 
-size_t packed_lds(int threads, int blocks) {
+// LDS: theta, partial dot products and residuals of two tiles, and in the end 8 doubles a thread.
+size_t packed_lds(int threads, int blocks, int stride) {
   const size_t slots = (size_t)(threads / blocks);
-  return std::max((size_t)threads * 8, slots * kPR * ((size_t)blocks + 1)) * sizeof(double);
+  return std::max((size_t)threads * 8, (size_t)32 * stride + 2 * slots * kPR * ((size_t)blocks + 1)) *
+         sizeof(double);
 }
 
 // Workgroup and persistent grid of the passes over n rows of dcols columns held in 4 bits.
@@ -613,16 +628,19 @@ int plan_packed(plr_ctx* c, int64_t n) {
   c->var = &kBlockShape;  // unused by this path, kept non-null
   c->nch_rt = 1;
   const int blocks = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
+  const PackedFns* pf = &kPacked[blocks <= 64 ? 0 : blocks <= 256 ? 1 : 2];
+  c->packed_fns = pf;
   c->packed_threads = packed_workgroup(blocks);
   int occ = 1 << 30;
-  const packed_fn used[] = {
-      c->packed_sweeps ? kPackedDot[0] : kPackedGrad[0], c->packed_sweeps ? kPackedDot[1] : kPackedGrad[1],
-      c->packed_sweeps ? kPackedAxpy[0] : kPackedEval, c->packed_sweeps ? kPackedAxpy[1] : kPackedEval};
-  for (packed_fn f : used) {
+  const packed_fn fused[] = {pf->grad[0], pf->grad[1], pf->eval};
+  const packed_fn sweeps[] = {kPackedDot[0], kPackedDot[1], kPackedAxpy[0], kPackedAxpy[1]};
+  const packed_fn* used = c->packed_sweeps ? sweeps : fused;
+  for (int k = 0; k < (c->packed_sweeps ? 4 : 3); ++k) {
+    const void* f = reinterpret_cast<const void*>(used[k]);
+    PLR_HIP(c, hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
     int o = 0;
     PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(
-                   &o, reinterpret_cast<const void*>(f), c->packed_threads,
-                   packed_lds(c->packed_threads, blocks)));
+                   &o, f, c->packed_threads, packed_lds(c->packed_threads, blocks, pf->stride)));
     occ = std::min(occ, o);
   }
   if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
@@ -805,16 +823,15 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
     a.blk0 = blk0;
     a.blocks = blocks;
     a.slots = threads / blocks;
-    // each row's partials are summed by as many threads as the tile's rows leave to each
+    // a lane sums at most 16 of a row's partials
     a.lanes_per_row = 1;
-    while (a.lanes_per_row < 64 && a.lanes_per_row < blocks &&
-           2 * a.lanes_per_row * a.slots * kPR <= threads)
-      a.lanes_per_row *= 2;
-    hipLaunchKernelGGL(f, dim3(c->grid), dim3(threads), packed_lds(threads, blocks), c->stream, a);
+    while (a.lanes_per_row < plr::kWave && a.lanes_per_row * 16 < blocks) a.lanes_per_row *= 2;
+    hipLaunchKernelGGL(f, dim3(c->grid), dim3(threads),
+                       packed_lds(threads, blocks, c->packed_fns->stride), c->stream, a);
     return hipGetLastError();
   };
   if (!c->packed_sweeps) {
-    PLR_HIP(c, launch(grad ? kPackedGrad[drop] : kPackedEval, 0, (int)c->row_blocks, c->packed_threads));
+    PLR_HIP(c, launch(grad ? c->packed_fns->grad[drop] : c->packed_fns->eval, 0, (int)c->row_blocks, c->packed_threads));
     *loss_parts = c->grid;
     return PLR_OK;
   }

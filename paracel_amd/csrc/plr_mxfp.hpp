@@ -28,33 +28,66 @@ struct Mask {
   int64_t row0;  // added to the row numbers of the launch
 };
 
-__device__ __forceinline__ void philox_round(unsigned (&c)[4], unsigned k0, unsigned k1) {
-  const uint64_t p = (uint64_t)c[0] * 0xD2511F53u, q = (uint64_t)c[2] * 0xCD9E8D57u;
-  const unsigned c1 = c[1], c3 = c[3];
-  c[0] = (unsigned)(q >> 32) ^ c1 ^ k0;
-  c[1] = (unsigned)q;
-  c[2] = (unsigned)(p >> 32) ^ c3 ^ k1;
-  c[3] = (unsigned)p;
+constexpr unsigned kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u;
+constexpr unsigned kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+
+__device__ __forceinline__ unsigned xor3(unsigned a, unsigned b, unsigned c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
 }
 
-// The keep bits of columns 8 * group .. 8 * group + 7 of a row (bit b: column 8 * group + b).
-__device__ __forceinline__ unsigned keep8(const Mask& m, int64_t row, unsigned group) {
+// The generator's first two rounds split into what depends on the column group alone and on the
+// row alone (half of the counter each): a kernel that meets a group in many rows, or a row in
+// several groups, makes each part once, and eight rounds are left per 8 values.
+struct MaskGroup {
+  unsigned a, b, c;
+};
+struct MaskRow {
+  unsigned a, b, c;
+};
+__device__ __forceinline__ MaskGroup mask_group(const Mask& m, unsigned group) {
+  const uint64_t p = (uint64_t)group * kPhiloxM0;
+  const uint64_t q = (uint64_t)((unsigned)(p >> 32) ^ m.step ^ m.key1) * kPhiloxM1;
+  return {(unsigned)(q >> 32) ^ (m.key0 + kPhiloxW0), (unsigned)q, (unsigned)p};
+}
+__device__ __forceinline__ MaskRow mask_row(const Mask& m, int64_t row) {
   const uint64_t r = (uint64_t)(row + m.row0);
-  unsigned c[4] = {group, (unsigned)r, (unsigned)(r >> 32), m.step};
-  unsigned k0 = m.key0, k1 = m.key1;
+  const uint64_t q = (uint64_t)(unsigned)(r >> 32) * kPhiloxM1;
+  const uint64_t p = (uint64_t)xor3((unsigned)(q >> 32), (unsigned)r, m.key0) * kPhiloxM0;
+  return {(unsigned)q, (unsigned)(p >> 32) ^ (m.key1 + kPhiloxW1), (unsigned)p};
+}
+
+typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
+
+// Mask of the 8 values of a group in a row: nibble i is 0xF where value i is kept, 0 where not.
+__device__ __forceinline__ unsigned keep_nibbles(const Mask& m, const MaskGroup& g, const MaskRow& r) {
+  unsigned c0 = g.a ^ r.a, c1 = g.b, c2 = r.b ^ g.c, c3 = r.c;
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    philox_round(c, k0, k1);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+  for (int i = 2; i < 10; ++i) {
+    const uint64_t p = (uint64_t)c0 * kPhiloxM0, q = (uint64_t)c2 * kPhiloxM1;
+    c0 = xor3((unsigned)(q >> 32), c1, m.key0 + (unsigned)i * kPhiloxW0);
+    c2 = xor3((unsigned)(p >> 32), c3, m.key1 + (unsigned)i * kPhiloxW1);
+    c1 = (unsigned)q;
+    c3 = (unsigned)p;
   }
-  unsigned bits = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    bits |= ((c[w] & 0xffffu) >= m.threshold ? 1u : 0u) << (2 * w);
-    bits |= ((c[w] >> 16) >= m.threshold ? 1u : 0u) << (2 * w + 1);
-  }
-  return bits;
+  // threshold - word, not below 0, is 0 where the value is kept; at most 1 of it marks a drop
+  const v2u16 t = {(unsigned short)m.threshold, (unsigned short)m.threshold}, one = {1, 1};
+  auto drops = [&](unsigned w) {
+    const v2u16 d = __builtin_elementwise_min(
+        __builtin_elementwise_sub_sat(t, __builtin_bit_cast(v2u16, w)), one);
+    return __builtin_bit_cast(unsigned, d);
+  };
+  // bytes 0 and 2 of each word hold a mark: the even values' go to the bytes of one word, the
+  // odd ones' to another's
+  const unsigned d0 = drops(c0), d1 = drops(c1), d2 = drops(c2), d3 = drops(c3);
+  const unsigned lo = __builtin_amdgcn_perm(d1, d0, 0x06020400u);  // d0.0 d1.0 d0.2 d1.2
+  const unsigned hi = __builtin_amdgcn_perm(d3, d2, 0x06020400u);
+  const unsigned even = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  const unsigned odd = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+  const unsigned marks = even | odd << 4;
+  return ~((marks << 4) - marks);
+}
+__device__ __forceinline__ unsigned keep_nibbles(const Mask& m, int64_t row, unsigned group) {
+  return keep_nibbles(m, mask_group(m, group), mask_row(m, row));
 }
 
 // 2^(s - 127) for a scale byte below 255 (s = 0 is the subnormal 2^-127).

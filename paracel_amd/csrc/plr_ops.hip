@@ -163,6 +163,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
   const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
   const int64_t c = chunk * 128 + l16 * 8;
   const T* x = static_cast<const T*>(a.x);
+  const MaskGroup group = DROP ? mask_group(a.mask, (unsigned)(c >> 3)) : MaskGroup{};
   Pack<T, 8> in[kQuantRows];
 #pragma unroll
   for (int u = 0; u < kQuantRows; ++u) {
@@ -175,11 +176,11 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
     if (r >= a.n) continue;  // (a quad shares its row: its lanes leave together)
     W v[8];
     unsigned top = 0;
-    const unsigned keep = DROP ? keep8(a.mask, r, (unsigned)(c >> 3)) : 0xffu;
+    const unsigned keep = DROP ? keep_nibbles(a.mask, group, mask_row(a.mask, r)) : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = Elem<T>::up(in[u].v[i]);
-      if (DROP && !(keep >> i & 1)) v[i] = W(0);
+      if (DROP && !(keep >> 4 * i & 1)) v[i] = W(0);
       const unsigned b = mag_bits(v[i]);
       top = b > top ? b : top;
     }
@@ -219,12 +220,13 @@ __global__ __launch_bounds__(64) void quantize_columns(QuantArgs a) {
     }
   }
   if (DROP) {
+    const MaskGroup group = mask_group(a.mask, (unsigned)(c0 >> 3));
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const unsigned keep = keep8(a.mask, r0 + i, (unsigned)(c0 >> 3)) >> (c0 & 7);
+      const unsigned keep = keep_nibbles(a.mask, group, mask_row(a.mask, r0 + i)) >> 4 * (c0 & 7);
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        if (!(keep >> k & 1)) in[i].v[k] = T(0);
+        if (!(keep >> 4 * k & 1)) in[i].v[k] = T(0);
     }
   }
 #pragma unroll
@@ -327,15 +329,16 @@ __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
     if (r < a.n) in[u] = load_pack<T, 8>(static_cast<const T*>(a.x) + r * a.ldx, c, a.d, a.wide_load);
   }
   const W sc = (W)a.scale;
+  const MaskGroup group = mask_group(a.mask, (unsigned)(c >> 3));
 #pragma unroll
   for (int u = 0; u < kQuantRows; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;
-    const unsigned keep = keep8(a.mask, r, (unsigned)(c >> 3));
+    const unsigned keep = keep_nibbles(a.mask, group, mask_row(a.mask, r));
     Pack<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      o.v[i] = (keep >> i & 1) ? Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc) : T(0);
+      o.v[i] = (keep >> 4 * i & 1) ? Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc) : T(0);
     store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
   }
 }

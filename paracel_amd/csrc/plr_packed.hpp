@@ -2,13 +2,19 @@
 // products, sigmoid, residual, loss and gradient of plr_kernels.hpp's passes on 17/32 of a byte
 // per value instead of 8, optionally with dropout of the values, arithmetic in 64 bits.
 //
-// A thread owns one block of 32 columns: its theta and its gradient sums stay in registers for
-// the kernel's lifetime, a row's 32 values are 16 bytes.  A workgroup lays G = threads / blocks
-// consecutive rows side by side (slots), and R such row sets make a tile.  A tile takes two
-// barriers: every thread's partial dot products go to LDS, are summed per row in a fixed order by
-// the threads of the workgroup, which evaluate the row terms, and the residuals come back through
-// LDS to the threads, whose codes -- and keep bits -- are still in registers.  No atomics: results
-// are reproducible bit for bit.
+// A thread owns one block of 32 columns: its gradient sums stay in registers for the kernel's
+// lifetime, theta in LDS (with it in registers too the compiler spills, 256 are all there are at
+// two waves per SIMD), a row's 32 values are 16 bytes.  A workgroup lays G = threads / blocks
+// consecutive rows side by side (slots), and R such row sets make a tile.  In step t
+//   1. every thread forms its partial dot products of tile t and leaves them in LDS,
+//   2. -- the step's one barrier --
+//   3. one wave (another one each step) sums the partials of tile t per row, in a fixed order,
+//      evaluates the row terms once per row and leaves the residuals in LDS,
+//   4. meanwhile every thread adds tile t - 1 to its gradient sums: those residuals are a step
+//      old, and the tile's codes are still in registers,
+//   5. the loads of tile t + 2 leave, tile t + 1 has arrived.
+// Dropout zeroes the codes when they arrive, so both uses meet the same values.  No atomics:
+// results are reproducible bit for bit.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -44,122 +50,225 @@ struct PackedArgs {
   plr_mx::Mask mask;
 };
 
-// The 32 values of a block times `t`, or added into `t` times w.
-template <bool DROP, typename F>
-__device__ __forceinline__ void each_value(uint4 codes, unsigned keep, F&& f) {
-  const unsigned w[4] = {codes.x, codes.y, codes.z, codes.w};
+constexpr int kPackedMaxThreads = 512;
+constexpr int kPackedRows = 4;  // R
+
+// R rows' codes of a thread's block, and their scale bytes in one word.
+template <int R>
+struct PackedTile {
+  uint4 codes[R];
+  unsigned scales;
+  static_assert(R <= 4, "a byte per row");
+};
+
+// The compiler must not carry the decoded values of a tile from its first use to its second:
+// 8 bytes per value instead of half a byte.
+template <int R>
+__device__ __forceinline__ void forget_decoded(PackedTile<R>& t) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    asm volatile("" : "+v"(t.codes[r].x), "+v"(t.codes[r].y), "+v"(t.codes[r].z), "+v"(t.codes[r].w));
+}
+
+// f(i, row, values of columns 2i and 2i + 1) for the R * 32 values of a tile, unscaled.
+template <int R, typename F>
+__device__ __forceinline__ void each_value(const PackedTile<R>& t, F&& f) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    plr_mx::v2f v[4] = {plr_mx::decode2<0>(w[q]), plr_mx::decode2<1>(w[q]),
-                        plr_mx::decode2<2>(w[q]), plr_mx::decode2<3>(w[q])};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x = v[i >> 1][i & 1];
-      if (DROP && !(keep >> (8 * q + i) & 1u)) x = 0.f;
-      f(8 * q + i, (double)x);
+    for (int p = 0; p < 4; ++p) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const unsigned w = q == 0 ? t.codes[r].x : q == 1 ? t.codes[r].y : q == 2 ? t.codes[r].z : t.codes[r].w;
+        const plr_mx::v2f v = p == 0   ? plr_mx::decode2<0>(w)
+                              : p == 1 ? plr_mx::decode2<1>(w)
+                              : p == 2 ? plr_mx::decode2<2>(w)
+                                       : plr_mx::decode2<3>(w);
+        f(4 * q + p, r, (double)v[0], (double)v[1]);
+      }
     }
   }
 }
 
-constexpr int kPackedMaxThreads = 512;
-constexpr int kPackedRows = 4;  // R
+// 2^(s - 127) of row r; a block that stands for NaN makes its row's dot product NaN.
+template <int R>
+__device__ __forceinline__ double tile_scale(const PackedTile<R>& t, int r) {
+  const unsigned s = t.scales >> (8 * r) & 255u;
+  return s == 255u ? __builtin_nan("") : plr_mx::scale_value_f64(s);
+}
 
-template <bool GRAD, bool DROP, int MODE, int R>
+// STRIDE: entries between theta's column pairs in LDS, at least `blocks` (fixed, so that a thread's
+// reads share one address).
+template <bool GRAD, bool DROP, int MODE, int STRIDE, int R = kPackedRows>
 __global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a) {
   extern __shared__ double sm[];
-  double* const zl = sm;                                     // [slots * R][blocks]
-  double* const rl = sm + (size_t)a.slots * R * a.blocks;    // [slots * R]
   const int tid = threadIdx.x, nt = blockDim.x;
+  const int rows = a.slots * R;  // rows of a tile
+  v2d* const thl = reinterpret_cast<v2d*>(sm);              // [16][STRIDE]: columns 2i, 2i + 1
+  double* const zl = sm + (MODE == kPassAxpy ? 0 : 32 * STRIDE);  // [2][rows][blocks]
+  double* const rl = zl + (size_t)2 * rows * a.blocks;      // [2][rows]
   const int slot = tid / a.blocks, blk = tid - slot * a.blocks;
   const bool active = slot < a.slots;
-  const int rows = a.slots * R;  // rows of a tile
-  double th[32], acc[32];
+  const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int nwaves = nt / kWave;
+  double acc[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    th[i] = active && MODE != kPassAxpy ? a.theta[(int64_t)(a.blk0 + blk) * 32 + i] : 0.;
-    acc[i] = 0.;
+  for (int i = 0; i < 32; ++i) acc[i] = 0.;
+  if (MODE != kPassAxpy) {
+    const v2d* src = reinterpret_cast<const v2d*>(a.theta + (int64_t)a.blk0 * 32);
+    for (int e = tid; e < 16 * a.blocks; e += nt) thl[(e & 15) * STRIDE + (e >> 4)] = src[e];
+    __syncthreads();
+  }
+  plr_mx::MaskGroup group[4];
+  if (DROP) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) group[q] = plr_mx::mask_group(a.mask, (unsigned)((a.blk0 + blk) * 4 + q));
   }
   RowSums sums;
   const double bias = a.theta_bias ? *a.theta_bias : 0.;
   const int64_t ntiles = (a.n + rows - 1) / rows;
-  for (int64_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-    const int64_t base = tile * rows;
-    uint4 codes[R];
-    unsigned sc[R], keep[R];
+
+  // Rows behind the last one, and threads without a block, read a row that is there and count
+  // nothing.
+  const unsigned at_lane = (unsigned)((active ? slot : 0) * a.row_blocks + a.blk0 + blk);
+  auto load = [&](int64_t tile, PackedTile<R>& t) {
+    t.scales = 0;
+    if ((tile + 1) * rows <= a.n) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int64_t at = (tile * rows + r * a.slots) * a.row_blocks;  // the same for all threads
+        t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
+        t.scales |= (unsigned)(a.scales + at)[at_lane] << (8 * r);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        int64_t row = tile * rows + r * a.slots + (active ? slot : 0);
+        row = row < a.n ? row : a.n - 1;
+        const int64_t at = row * a.row_blocks + a.blk0 + blk;
+        t.codes[r] = *reinterpret_cast<const uint4*>(a.codes + at * 16);
+        t.scales |= (unsigned)a.scales[at] << (8 * r);
+      }
+    }
+  };
+  auto drop = [&](int64_t tile, PackedTile<R>& t) {
+    if (!DROP) return;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r * a.slots + slot;
-      codes[r] = uint4{0, 0, 0, 0};
-      sc[r] = 127u;
-      if (active && row < a.n) {
-        const int64_t at = row * a.row_blocks + a.blk0 + blk;
-        codes[r] = *reinterpret_cast<const uint4*>(a.codes + at * 16);
-        sc[r] = a.scales[at];
-      }
+      const plr_mx::MaskRow mr = plr_mx::mask_row(a.mask, tile * rows + r * a.slots + slot);
+      t.codes[r].x &= plr_mx::keep_nibbles(a.mask, group[0], mr);
+      t.codes[r].y &= plr_mx::keep_nibbles(a.mask, group[1], mr);
+      t.codes[r].z &= plr_mx::keep_nibbles(a.mask, group[2], mr);
+      t.codes[r].w &= plr_mx::keep_nibbles(a.mask, group[3], mr);
     }
-    if (DROP) {
+  };
+  auto dot = [&](PackedTile<R>& t, double* z) {
+    double part[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        keep[r] = 0;
-        const int64_t row = base + r * a.slots + slot;
+    for (int r = 0; r < R; ++r) part[r] = 0.;
+    v2d th;
+    each_value<R>(t, [&](int i, int r, double x0, double x1) {
+      if (r == 0) th = thl[i * STRIDE + blk];
+      part[r] = fma(x0, th.x, part[r]);
+      part[r] = fma(x1, th.y, part[r]);
+      // here, and not all decoded first and summed behind the branch: that takes every register
+      asm volatile("" : "+v"(part[r]));
+    });
+    if (active) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          keep[r] |= plr_mx::keep8(a.mask, row, (unsigned)((a.blk0 + blk) * 4 + q)) << (8 * q);
-      }
+      for (int r = 0; r < R; ++r)
+        z[(r * a.slots + slot) * a.blocks + blk] = part[r] * tile_scale(t, r);
     }
-    // 2^(s - 127); a block that stands for NaN makes its row's dot product NaN
-    double s64[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      s64[r] = sc[r] == 255u ? __builtin_nan("") : plr_mx::scale_value_f64(sc[r]);
-    if (MODE != kPassAxpy) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        double z = 0.;
-        each_value<DROP>(codes[r], DROP ? keep[r] : 0u, [&](int i, double x) { z = fma(x, th[i], z); });
-        if (active) zl[(r * a.slots + slot) * a.blocks + blk] = z * s64[r];
+  };
+  // Row sums and row terms: `per` lanes share a row, a wave takes 64 / per rows at a time, the
+  // waves take turns from tile to tile.
+  auto finish_rows = [&](int64_t tile, const double* z, double* res) {
+    const int per = a.lanes_per_row, step = kWave / per, sub = lane & (per - 1);
+    int first = wave - (int)(tile % nwaves);
+    if (first < 0) first += nwaves;
+    for (int q0 = first * step; q0 < rows; q0 += nwaves * step) {
+      const int q = q0 + lane / per;
+      double s = 0.;
+      if (q < rows) {
+        const double* p = z + (size_t)q * a.blocks;
+#pragma unroll 4
+        for (int b = sub; b < a.blocks; b += per) s += p[b];
       }
-      __syncthreads();
-      const int P = a.lanes_per_row;
-      const int sub = tid & (P - 1);
-      for (int q0 = 0; q0 < rows; q0 += nt / P) {
-        const int q = q0 + tid / P;
-        double z = 0.;
-        if (q < rows)
-          for (int b = sub; b < a.blocks; b += P) z += zl[q * a.blocks + b];
-        for (int m = 1; m < P; m <<= 1) z += __shfl_xor(z, m, kWave);
-        const int64_t row = base + q;
-        if (q < rows && sub == 0) {
-          double res = 0.;
-          if (row < a.n) {
-            if (DROP) z *= a.kept;
-            if (MODE == kPassDot) {
-              a.z_buf[row] = a.z_accumulate ? a.z_buf[row] + z : z;
-            } else {
-              double h, l;
-              const double yv = a.y ? a.y[row] : 0.;
-              row_terms(z + bias, yv, a.loss_mode, a.identity_link, h, l);
-              sums.loss += l;
-              res = h - yv;
-              sums.res += res;
-              if (a.h_out) store_h(a.h_out + row, h);
-            }
+      for (int m = 1; m < per; m <<= 1) s += __shfl_xor(s, m, kWave);
+      const int64_t row = tile * rows + q;
+      if (q < rows && sub == 0) {
+        double rv = 0.;
+        if (row < a.n) {
+          if (DROP) s *= a.kept;
+          if (MODE == kPassDot) {
+            a.z_buf[row] = a.z_accumulate ? a.z_buf[row] + s : s;
+          } else {
+            double h, l;
+            const double yv = a.y ? a.y[row] : 0.;
+            row_terms(s + bias, yv, a.loss_mode, a.identity_link, h, l);
+            sums.loss += l;
+            rv = h - yv;
+            sums.res += rv;
+            if (a.h_out) store_h(a.h_out + row, h);
           }
-          if (GRAD) rl[q] = res;
         }
+        if (GRAD) res[q] = rv;
       }
-      __syncthreads();
     }
-    if (GRAD) {
+  };
+  auto update = [&](PackedTile<R>& t, const double* w) {
+    each_value<R>(t, [&](int i, int r, double x0, double x1) {
+      acc[2 * i] = fma(x0, w[r], acc[2 * i]);
+      acc[2 * i + 1] = fma(x1, w[r], acc[2 * i + 1]);
+    });
+  };
+
+  const int64_t t0 = blockIdx.x, dt = gridDim.x;
+  if (MODE == kPassAxpy) {
+    PackedTile<R> cur, nxt;
+    if (t0 < ntiles) load(t0, nxt);
+    for (int64_t t = t0; t < ntiles; t += dt) {
+      cur = nxt;
+      if (t + dt < ntiles) load(t + dt, nxt);
+      drop(t, cur);
+      double w[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int64_t row = base + r * a.slots + slot;
-        double w = 0.;
-        if (active && row < a.n) w = MODE == kPassAxpy ? a.res_in[row] : rl[r * a.slots + slot];
-        w *= DROP ? s64[r] * a.kept : s64[r];
-        each_value<DROP>(codes[r], DROP ? keep[r] : 0u,
-                         [&](int i, double x) { acc[i] = fma(x, w, acc[i]); });
+        const int64_t row = t * rows + r * a.slots + slot;
+        w[r] = active && row < a.n ? a.res_in[row] * tile_scale(cur, r) : 0.;
+        if (DROP) w[r] *= a.kept;
       }
+      update(cur, w);
+    }
+  } else {
+    PackedTile<R> prev, cur, nxt;
+    if (t0 < ntiles) load(t0, cur);
+    if (t0 + dt < ntiles) load(t0 + dt, nxt);
+    int par = 0;
+    for (int64_t t = t0; t < ntiles + (GRAD ? dt : 0); t += dt, par ^= 1) {
+      const bool live = t < ntiles;  // (with a gradient the last step only adds the last tile)
+      if (live) {
+        drop(t, cur);
+        dot(cur, zl + (size_t)par * rows * a.blocks);
+      }
+      __syncthreads();
+      if (live) finish_rows(t, zl + (size_t)par * rows * a.blocks, rl + par * rows);
+      if (GRAD) {
+        if (t >= t0 + dt) {
+          forget_decoded(prev);
+          const double* res = rl + (par ^ 1) * rows;
+          double w[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            w[r] = active ? res[r * a.slots + slot] * tile_scale(prev, r) : 0.;
+            if (DROP) w[r] *= a.kept;
+          }
+          update(prev, w);
+        }
+        prev = cur;
+      }
+      cur = nxt;
+      if (t + 2 * dt < ntiles) load(t + 2 * dt, nxt);
     }
   }
   if (GRAD) {
@@ -182,17 +291,17 @@ __global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a
     }
   }
   if (MODE == kPassFused) {
-    // the waves' loss and residual sums, in wave order (waves beyond the workgroup's count as 0)
+    // the waves' loss and residual sums, in wave order
     __shared__ double lx[kPackedMaxThreads / kWave], rx[kPackedMaxThreads / kWave];
     const double wl = wave_sum(sums.loss), wr = wave_sum(sums.res);
-    if ((tid & 63) == 0) {
-      lx[tid >> 6] = wl;
-      rx[tid >> 6] = wr;
+    if (lane == 0) {
+      lx[wave] = wl;
+      rx[wave] = wr;
     }
     __syncthreads();
     if (tid == 0) {
       double l = 0., r = 0.;
-      for (int w = 0; w < nt / kWave; ++w) {
+      for (int w = 0; w < nwaves; ++w) {
         l += lx[w];
         r += rx[w];
       }
