@@ -219,22 +219,28 @@ std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 typedef void (*packed_fn)(plr::PackedArgs);
 struct PackedFns {
   int stride;         // blocks of theta in LDS: the widest row
+  int sets;           // row sets of a tile
+  int threads;
   packed_fn grad[2];  // [dropout]
   packed_fn eval;
 };
-template <int STRIDE>
+template <int STRIDE, int SR, int NT, int MINW>
 constexpr PackedFns make_packed() {
-  return {STRIDE,
-          {plr::packed_pass<true, false, plr::kPassFused, STRIDE>,
-           plr::packed_pass<true, true, plr::kPassFused, STRIDE>},
-          plr::packed_pass<false, false, plr::kPassFused, STRIDE>};
+  return {STRIDE, SR, NT,
+          {plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>,
+           plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
+          plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>};
 }
-const PackedFns kPacked[3] = {make_packed<64>(), make_packed<256>(), make_packed<512>()};
-const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, 256>,
-                                 plr::packed_pass<false, true, plr::kPassDot, 256>};
-const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, 256>,
-                                  plr::packed_pass<true, true, plr::kPassAxpy, 256>};
-constexpr int kPR = plr::kPackedRows;
+// Row sets per tile: as many as leave two workgroups (of 512 threads one) on a compute unit; the
+// barriers and row terms of a tile cost the same however long it is (1M x 1000: 16 sets 265 us,
+// 8 sets 301).  Rows of up to 8 blocks lie 32 and more side by side: with 8 sets their partials
+// stay small enough (1M x 100 with dropout: 8 sets 80 us, 16 sets 92).
+const PackedFns kPacked[4] = {make_packed<8, 8, 256, 2>(), make_packed<64, 16, 256, 2>(),
+                              make_packed<256, 8, 512, 2>(), make_packed<512, 4, 512, 2>()};
+const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, 256, 8, 512, 2>,
+                                 plr::packed_pass<false, true, plr::kPassDot, 256, 8, 512, 2>};
+const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, 256, 8, 512, 2>,
+                                  plr::packed_pass<true, true, plr::kPassAxpy, 256, 8, 512, 2>};
 constexpr int kPackedFused = 480, kPackedPiece = 256;
 
 }  // namespace
@@ -343,7 +349,7 @@ struct plr_ctx {
   uint8_t* d_scales = nullptr;    // n x row_blocks
   int64_t row_blocks = 0;
   const PackedFns* packed_fns = nullptr;
-  int packed_threads = 0;
+  int packed_grid[3] = {0, 0, 0};  // a gradient, one with dropout, none
   bool packed_sweeps = false;     // too wide for one read: column pieces, two sweeps
   bool drop_on = false;           // plr_set_dropout
   plr_dropout drop = {0., 0, 0, 0};
@@ -390,7 +396,6 @@ void free_shape(plr_ctx* c) {
   c->d_codes = c->d_scales = nullptr;
   c->packed = c->packed_sweeps = false;
   c->row_blocks = 0;
-  c->packed_threads = 0;
   if (c->dy) (void)hipFree(c->dy);
   if (c->d_theta) (void)hipFree(c->d_theta);
   if (c->d_part_g) (void)hipFree(c->d_part_g);
@@ -606,18 +611,33 @@ int plan_shape(plr_ctx* c, int64_t n, int64_t d) {
   return PLR_OK;
 }
 
-// Threads of a workgroup for rows of `blocks` blocks: two workgroups of 256 per compute unit or
-// one of 512, whichever leaves fewer threads idle.
-int packed_workgroup(int blocks) {
-  if (blocks > 64) return 512;
-  return (512 / blocks) > 2 * (256 / blocks) ? 512 : 256;
+// Rows side by side.  (A narrow last piece of a wide row does not need every thread, and what is
+// read behind the last row stays short.)
+int packed_slots(const PackedFns* f, int blocks) {
+  return std::min(f->threads / blocks, f->stride == kPackedPiece ? 64 : f->threads);
 }
 
-// LDS: theta, partial dot products and residuals of two tiles, and in the end 8 doubles a thread.
-size_t packed_lds(int threads, int blocks, int stride) {
-  const size_t slots = (size_t)(threads / blocks);
-  return std::max((size_t)threads * 8, (size_t)32 * stride + 2 * slots * kPR * ((size_t)blocks + 1)) *
-         sizeof(double);
+// LDS: theta, partial dot products, residuals and (with dropout) marks of a tile, and in the end
+// 8 doubles a thread.
+size_t packed_lds(const PackedFns* f, int blocks, bool drop) {
+  const size_t rows = (size_t)packed_slots(f, blocks) * f->sets;
+  return std::max((size_t)f->threads * 8, (size_t)32 * f->stride + rows * ((blocks | 1) + 1)) *
+             sizeof(double) + (drop ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
+}
+
+const PackedFns* packed_fns_for(int64_t blocks) {
+  return &kPacked[blocks <= 8                                  ? 0
+                  : blocks <= 64                               ? 1
+                  : blocks <= 256 || blocks > kPackedFused ? 2
+                                                               : 3];
+}
+
+// Rows the kernels may read behind the last one: less than a group of row sets of any launch.
+int64_t packed_slack_rows(int64_t row_blocks) {
+  const PackedFns* f = packed_fns_for(row_blocks);
+  const int64_t least = row_blocks > kPackedFused && row_blocks % kPackedPiece
+                            ? row_blocks % kPackedPiece : std::min<int64_t>(row_blocks, kPackedPiece);
+  return (int64_t)packed_slots(f, (int)(row_blocks > kPackedFused ? least : row_blocks)) * plr::kPackedR;
 }
 
 // Workgroup and persistent grid of the passes over n rows of dcols columns held in 4 bits.
@@ -628,31 +648,36 @@ int plan_packed(plr_ctx* c, int64_t n) {
   c->var = &kBlockShape;  // unused by this path, kept non-null
   c->nch_rt = 1;
   const int blocks = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
-  const PackedFns* pf = &kPacked[blocks <= 64 ? 0 : blocks <= 256 ? 1 : 2];
+  const PackedFns* pf = packed_fns_for(blocks);
   c->packed_fns = pf;
-  c->packed_threads = packed_workgroup(blocks);
-  int occ = 1 << 30;
-  const packed_fn fused[] = {pf->grad[0], pf->grad[1], pf->eval};
-  const packed_fn sweeps[] = {kPackedDot[0], kPackedDot[1], kPackedAxpy[0], kPackedAxpy[1]};
-  const packed_fn* used = c->packed_sweeps ? sweeps : fused;
-  for (int k = 0; k < (c->packed_sweeps ? 4 : 3); ++k) {
-    const void* f = reinterpret_cast<const void*>(used[k]);
-    PLR_HIP(c, hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
-    int o = 0;
-    PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(
-                   &o, f, c->packed_threads, packed_lds(c->packed_threads, blocks, pf->stride)));
-    occ = std::min(occ, o);
+  const int64_t groups = ceil_div(n, (int64_t)packed_slots(pf, blocks) * plr::kPackedR);
+  // [without dropout, with it, without a gradient]: the instances that a pass of that kind launches
+  const packed_fn used[3][2] = {{pf->grad[0], pf->grad[0]}, {pf->grad[1], pf->grad[1]},
+                                {pf->eval, pf->eval}};
+  const packed_fn sweeps[3][2] = {{kPackedDot[0], kPackedAxpy[0]}, {kPackedDot[1], kPackedAxpy[1]},
+                                  {kPackedDot[0], kPackedDot[0]}};
+  for (int k = 0; k < 3; ++k) {
+    int occ = 1 << 30;
+    for (int i = 0; i < 2; ++i) {
+      const void* f = reinterpret_cast<const void*>(c->packed_sweeps ? sweeps[k][i] : used[k][i]);
+      PLR_HIP(c, hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
+      int o = 0;
+      PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(&o, f, pf->threads,
+                                                              packed_lds(pf, blocks, k == 1)));
+      occ = std::min(occ, o);
+    }
+    if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
+    c->packed_grid[k] = (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)c->num_cu * occ));
   }
-  if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
-  const int64_t tiles = ceil_div(n, (int64_t)(c->packed_threads / blocks) * kPR);
-  c->grid = c->grid_nograd =
-      (int)std::max<int64_t>(1, std::min<int64_t>(tiles, (int64_t)c->num_cu * occ));
+  c->grid = std::max(c->packed_grid[0], c->packed_grid[1]);
+  c->grid_nograd = c->packed_grid[2];
   char b[256];
   snprintf(b, sizeof b,
-           "packed_pass<R=%d> 4-bit shard, %lld blocks of 32 columns per row%s, %d rows side by side, "
-           "grid=%d x %d threads (occupancy %d blocks/CU, %d CUs)",
-           kPR, (long long)c->row_blocks, c->packed_sweeps ? " in pieces of 256, two sweeps" : "",
-           c->packed_threads / blocks, c->grid, c->packed_threads, occ, c->num_cu);
+           "packed_pass<SR=%d> 4-bit shard, %lld blocks of 32 columns per row%s, %d rows side by side, "
+           "grid=%d x %d threads (%d with dropout, %d without a gradient)",
+           pf->sets, (long long)c->row_blocks, c->packed_sweeps ? " in pieces of 256, two sweeps" : "",
+           packed_slots(pf, blocks), c->packed_grid[0], pf->threads, c->packed_grid[1],
+           c->packed_grid[2]);
   c->info = b;
   if (c->bias) c->info += "; first column constant 1, not stored";
   return PLR_OK;
@@ -789,9 +814,10 @@ int upload_rows(plr_ctx* c, int64_t row0, int64_t nrows, const double* X,
 
 enum PassKind { kPassGrad, kPassDelta, kPassLoss, kPassPredict, kPassPredictLinear };
 
-// The streaming kernels of a pass over a shard held in 4 bits.  *loss_parts: how many partial
-// losses they leave.
-int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, int* loss_parts) {
+// The streaming kernels of a pass over a shard held in 4 bits.  *parts and *loss_parts: how many
+// partial gradients and losses they leave.
+int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, int* parts,
+                   int* loss_parts) {
   plr::PackedArgs a;
   a.codes = c->d_codes;
   a.scales = c->d_scales;
@@ -819,26 +845,28 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
     a.mask = plr_mx::Mask{t, (unsigned)c->drop.seed, (unsigned)(c->drop.seed >> 32),
                           c->drop.step + (unsigned)std::max(train_round, 0), c->drop.row0};
   }
-  auto launch = [&](packed_fn f, int blk0, int blocks, int threads) {
+  const PackedFns* pf = c->packed_fns;
+  const int grid = c->packed_grid[!grad ? 2 : drop ? 1 : 0];
+  *parts = *loss_parts = grid;
+  auto launch = [&](packed_fn f, int blk0, int blocks) {
     a.blk0 = blk0;
     a.blocks = blocks;
-    a.slots = threads / blocks;
-    // a lane sums at most 16 of a row's partials
+    a.slots = packed_slots(pf, blocks);
+    a.groups = ceil_div(c->n, (int64_t)a.slots * plr::kPackedR);
+    // a lane sums up to 32 of a row's partials: the fewer waves evaluate row terms the better
     a.lanes_per_row = 1;
-    while (a.lanes_per_row < plr::kWave && a.lanes_per_row * 16 < blocks) a.lanes_per_row *= 2;
-    hipLaunchKernelGGL(f, dim3(c->grid), dim3(threads),
-                       packed_lds(threads, blocks, c->packed_fns->stride), c->stream, a);
+    while (a.lanes_per_row < plr::kWave && a.lanes_per_row * 32 < blocks) a.lanes_per_row *= 2;
+    hipLaunchKernelGGL(f, dim3(grid), dim3(pf->threads), packed_lds(pf, blocks, drop), c->stream, a);
     return hipGetLastError();
   };
   if (!c->packed_sweeps) {
-    PLR_HIP(c, launch(grad ? c->packed_fns->grad[drop] : c->packed_fns->eval, 0, (int)c->row_blocks, c->packed_threads));
-    *loss_parts = c->grid;
+    PLR_HIP(c, launch(grad ? c->packed_fns->grad[drop] : c->packed_fns->eval, 0, (int)c->row_blocks));
     return PLR_OK;
   }
   for (int64_t b = 0; b < c->row_blocks; b += kPackedPiece) {
     const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
     a.z_accumulate = b > 0;
-    PLR_HIP(c, launch(kPackedDot[drop], (int)b, w, c->packed_threads));
+    PLR_HIP(c, launch(kPackedDot[drop], (int)b, w));
   }
   hipLaunchKernelGGL(plr::residual_pass, dim3(c->res_grid), dim3(256), 0, c->stream,
                      (const double*)c->d_z, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
@@ -848,7 +876,7 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
   *loss_parts = c->res_grid;
   for (int64_t b = 0; grad && b < c->row_blocks; b += kPackedPiece) {
     const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
-    PLR_HIP(c, launch(kPackedAxpy[drop], (int)b, w, c->packed_threads));
+    PLR_HIP(c, launch(kPackedAxpy[drop], (int)b, w));
   }
   return PLR_OK;
 }
@@ -897,10 +925,10 @@ int enqueue_pass(plr_ctx* c, PassKind kind, unsigned loss_mode, double alpha, do
   pa.z_accumulate = 0;
   pa.res_in = nullptr;
 
-  int packed_parts = 0;
+  int packed_parts = 0, packed_loss_parts = 0;
   if (c->timing) PLR_HIP(c, hipEventRecord(c->ev0, c->stream));
   if (c->packed) {
-    const int rc = enqueue_packed(c, pa, grad, train_round, &packed_parts);
+    const int rc = enqueue_packed(c, pa, grad, train_round, &packed_parts, &packed_loss_parts);
     if (rc != PLR_OK) return rc;
   } else if (c->lane) {
     hipLaunchKernelGGL(c->lane->fn[grad ? 1 : 0], dim3(grid), dim3(threads), 0, c->stream, pa);
@@ -1017,8 +1045,8 @@ int enqueue_pass(plr_ctx* c, PassKind kind, unsigned loss_mode, double alpha, do
     fa.n = c->n;
     fa.part_res = pa.part_res;
     fa.theta_bias = c->d_theta + c->bias_slot;
-    fa.nparts = team ? c->nteams : grid;  // a team shares one row of partials
-    fa.nparts_loss = c->packed ? packed_parts : (team || team_dot) ? c->res_grid : grid;
+    fa.nparts = c->packed ? packed_parts : team ? c->nteams : grid;  // a team shares one row of partials
+    fa.nparts_loss = c->packed ? packed_loss_parts : (team || team_dot) ? c->res_grid : grid;
     fa.delta_mode = (kind == kPassDelta) ? (train_round >= 0 ? 2 : 1) : 0;
     fa.have_grad = grad ? 1 : 0;
     const int fblocks = grad ? (int)ceil_div(c->dcols, plr::kFinCols) : 1;
@@ -1827,8 +1855,12 @@ int plr_pack_data(plr_ctx* c) {
   const int64_t n = c->n, d = c->d, blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
   DevBuf codes, scales;
   if (n > 0) {
-    PLR_HIP(c, hipMalloc(&codes.p, (size_t)n * blocks * 16));
-    PLR_HIP(c, hipMalloc(&scales.p, (size_t)n * blocks));
+    // zeros behind the last row, which the kernels read
+    const size_t end = (size_t)n * blocks, slack = (size_t)packed_slack_rows(blocks) * blocks;
+    PLR_HIP(c, hipMalloc(&codes.p, (end + slack) * 16));
+    PLR_HIP(c, hipMalloc(&scales.p, end + slack));
+    PLR_HIP(c, hipMemsetAsync(static_cast<uint8_t*>(codes.p) + end * 16, 0, slack * 16, c->stream));
+    PLR_HIP(c, hipMemsetAsync(static_cast<uint8_t*>(scales.p) + end, 0, slack, c->stream));
     // rows as they lie, or, row-tiled ones, block by block through dense rows
     const int64_t chunk = c->lane ? std::max<int64_t>(1, (int64_t)(256u << 20) / (d * 8)) : n;
     DevBuf stage;

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void matmul_simple(MatmulArgs p) {
         const int64_t i = i0 + 16 * x + q * 4 + e, j = j0 + 16 * y + r16;
         if (i >= p.m || j >= p.n) continue;
         float v = p.alpha * acc[x][y][e];
-        if (DROP) v = (keep_nibbles(p.mask, i, (unsigned)(j >> 3)) >> 4 * (j & 7) & 1) ? v * p.kept : 0.f;
+        if (DROP) v = (drop_marks(p.mask, i, (unsigned)(j >> 3)) >> 4 * (j & 7) & 1) ? 0.f : v * p.kept;
         static_cast<T*>(p.c)[i * p.ldc + j] = narrow<T>(v);
       }
 }

@@ -56,10 +56,8 @@ __device__ __forceinline__ MaskRow mask_row(const Mask& m, int64_t row) {
   return {(unsigned)q, (unsigned)(p >> 32) ^ (m.key1 + kPhiloxW1), (unsigned)p};
 }
 
-typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
-
-// Mask of the 8 values of a group in a row: nibble i is 0xF where value i is kept, 0 where not.
-__device__ __forceinline__ unsigned keep_nibbles(const Mask& m, const MaskGroup& g, const MaskRow& r) {
+// The 8 values of a group in a row: bit 4 i is 1 where value i is dropped.
+__device__ __forceinline__ unsigned drop_marks(const Mask& m, const MaskGroup& g, const MaskRow& r) {
   unsigned c0 = g.a ^ r.a, c1 = g.b, c2 = r.b ^ g.c, c3 = r.c;
 #pragma unroll
   for (int i = 2; i < 10; ++i) {
@@ -69,12 +67,15 @@ __device__ __forceinline__ unsigned keep_nibbles(const Mask& m, const MaskGroup&
     c1 = (unsigned)q;
     c3 = (unsigned)p;
   }
-  // threshold - word, not below 0, is 0 where the value is kept; at most 1 of it marks a drop
-  const v2u16 t = {(unsigned short)m.threshold, (unsigned short)m.threshold}, one = {1, 1};
+  // threshold - word, not below 0, is 0 where the value is kept; at most 1 of it marks a drop.  (As
+  // instructions: from vector operations the compiler makes a comparison and a selection for
+  // every half word.)
+  const unsigned t = m.threshold | m.threshold << 16, one = 0x00010001u;
   auto drops = [&](unsigned w) {
-    const v2u16 d = __builtin_elementwise_min(
-        __builtin_elementwise_sub_sat(t, __builtin_bit_cast(v2u16, w)), one);
-    return __builtin_bit_cast(unsigned, d);
+    unsigned d;
+    asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(d) : "s"(t), "v"(w));
+    asm("v_pk_min_u16 %0, %1, %2" : "=v"(d) : "s"(one), "v"(d));
+    return d;
   };
   // bytes 0 and 2 of each word hold a mark: the even values' go to the bytes of one word, the
   // odd ones' to another's
@@ -83,11 +84,13 @@ __device__ __forceinline__ unsigned keep_nibbles(const Mask& m, const MaskGroup&
   const unsigned hi = __builtin_amdgcn_perm(d3, d2, 0x06020400u);
   const unsigned even = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   const unsigned odd = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-  const unsigned marks = even | odd << 4;
-  return ~((marks << 4) - marks);
+  return even | odd << 4;
 }
-__device__ __forceinline__ unsigned keep_nibbles(const Mask& m, int64_t row, unsigned group) {
-  return keep_nibbles(m, mask_group(m, group), mask_row(m, row));
+// Nibble i is 0xF where value i is kept, 0 where it is dropped.
+__device__ __forceinline__ unsigned kept_nibbles(unsigned marks) { return ~((marks << 4) - marks); }
+
+__device__ __forceinline__ unsigned drop_marks(const Mask& m, int64_t row, unsigned group) {
+  return drop_marks(m, mask_group(m, group), mask_row(m, row));
 }
 
 // 2^(s - 127) for a scale byte below 255 (s = 0 is the subnormal 2^-127).

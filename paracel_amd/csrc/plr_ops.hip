@@ -176,11 +176,11 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
     if (r >= a.n) continue;  // (a quad shares its row: its lanes leave together)
     W v[8];
     unsigned top = 0;
-    const unsigned keep = DROP ? keep_nibbles(a.mask, group, mask_row(a.mask, r)) : 0u;
+    const unsigned drop = DROP ? drop_marks(a.mask, group, mask_row(a.mask, r)) : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = Elem<T>::up(in[u].v[i]);
-      if (DROP && !(keep >> 4 * i & 1)) v[i] = W(0);
+      if (DROP && (drop >> 4 * i & 1)) v[i] = W(0);
       const unsigned b = mag_bits(v[i]);
       top = b > top ? b : top;
     }
@@ -223,10 +223,10 @@ __global__ __launch_bounds__(64) void quantize_columns(QuantArgs a) {
     const MaskGroup group = mask_group(a.mask, (unsigned)(c0 >> 3));
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const unsigned keep = keep_nibbles(a.mask, group, mask_row(a.mask, r0 + i)) >> 4 * (c0 & 7);
+      const unsigned drop = drop_marks(a.mask, group, mask_row(a.mask, r0 + i)) >> 4 * (c0 & 7);
 #pragma unroll
       for (int k = 0; k < V; ++k)
-        if (!(keep >> 4 * k & 1)) in[i].v[k] = T(0);
+        if (drop >> 4 * k & 1) in[i].v[k] = T(0);
     }
   }
 #pragma unroll
@@ -334,11 +334,11 @@ __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
   for (int u = 0; u < kQuantRows; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;
-    const unsigned keep = keep_nibbles(a.mask, group, mask_row(a.mask, r));
+    const unsigned drop = drop_marks(a.mask, group, mask_row(a.mask, r));
     Pack<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      o.v[i] = (keep >> 4 * i & 1) ? Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc) : T(0);
+      o.v[i] = (drop >> 4 * i & 1) ? T(0) : Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc);
     store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
   }
 }

@@ -2,19 +2,21 @@
 // products, sigmoid, residual, loss and gradient of plr_kernels.hpp's passes on 17/32 of a byte
 // per value instead of 8, optionally with dropout of the values, arithmetic in 64 bits.
 //
+// Bound by instructions, not bytes: a value costs two multiply-adds in 64 bits and 1.5
+// conversions for each of them, with dropout also an eighth of a generator call.
+//
 // A thread owns one block of 32 columns: its gradient sums stay in registers for the kernel's
-// lifetime, theta in LDS (with it in registers too the compiler spills, 256 are all there are at
-// two waves per SIMD), a row's 32 values are 16 bytes.  A workgroup lays G = threads / blocks
-// consecutive rows side by side (slots), and R such row sets make a tile.  In step t
-//   1. every thread forms its partial dot products of tile t and leaves them in LDS,
-//   2. -- the step's one barrier --
-//   3. one wave (another one each step) sums the partials of tile t per row, in a fixed order,
-//      evaluates the row terms once per row and leaves the residuals in LDS,
-//   4. meanwhile every thread adds tile t - 1 to its gradient sums: those residuals are a step
-//      old, and the tile's codes are still in registers,
-//   5. the loads of tile t + 2 leave, tile t + 1 has arrived.
-// Dropout zeroes the codes when they arrive, so both uses meet the same values.  No atomics:
-// results are reproducible bit for bit.
+// lifetime, theta is in LDS, a row's 32 values are 16 bytes.  A workgroup lays G = threads /
+// blocks consecutive rows side by side (slots) and takes SR such row sets to a tile:
+//   1. every thread forms its partial dot products of the tile, R row sets at a time, and leaves
+//      them in LDS (with dropout also a bit per value that says what was kept),
+//   2. the partials are summed per row in a fixed order and the row terms are evaluated, once per
+//      row; the residuals go to LDS,
+//   3. every thread reads the tile's codes again -- from the caches, a tile is 64 KB -- and adds
+//      them to its gradient sums.
+// Two barriers per tile.  The row terms are a chain of some 250 dependent instructions; with
+// short tiles (the codes kept in registers from 1 to 3) the workgroup spent half its time there.
+// No atomics: results are reproducible bit for bit.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -38,10 +40,11 @@ struct PackedArgs {
   double* z_buf;          // kPassDot: n
   const double* res_in;   // kPassAxpy: n
   int64_t n;
+  int64_t groups;         // of R row sets: ceil(n / (slots * R))
   int64_t row_blocks;     // blocks of a stored row
   int64_t pitch;          // doubles per row of part_g
   int blk0, blocks;       // the blocks this launch covers
-  int slots;              // rows side by side: blockDim / blocks
+  int slots;              // rows side by side: threads / blocks
   int lanes_per_row;      // threads that sum a row's partials (a power of two, at most 64)
   int z_accumulate;
   unsigned loss_mode;
@@ -49,9 +52,6 @@ struct PackedArgs {
   double kept;            // dropout: the factor of what is kept
   plr_mx::Mask mask;
 };
-
-constexpr int kPackedMaxThreads = 512;
-constexpr int kPackedRows = 4;  // R
 
 // R rows' codes of a thread's block, and their scale bytes in one word.
 template <int R>
@@ -61,33 +61,35 @@ struct PackedTile {
   static_assert(R <= 4, "a byte per row");
 };
 
-// The compiler must not carry the decoded values of a tile from its first use to its second:
-// 8 bytes per value instead of half a byte.
+// The same while its loads are under way (nothing may be computed from them yet).
 template <int R>
-__device__ __forceinline__ void forget_decoded(PackedTile<R>& t) {
+struct PackedLoads {
+  uint4 codes[R];
+  unsigned char scales[R];
+};
+template <int R>
+__device__ __forceinline__ PackedTile<R> arrived(const PackedLoads<R>& l) {
+  PackedTile<R> t;
+  t.scales = 0;
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    asm volatile("" : "+v"(t.codes[r].x), "+v"(t.codes[r].y), "+v"(t.codes[r].z), "+v"(t.codes[r].w));
+  for (int r = 0; r < R; ++r) {
+    t.codes[r] = l.codes[r];
+    t.scales |= (unsigned)l.scales[r] << (8 * r);
+  }
+  return t;
 }
 
-// f(i, row, values of columns 2i and 2i + 1) for the R * 32 values of a tile, unscaled.
-template <int R, typename F>
-__device__ __forceinline__ void each_value(const PackedTile<R>& t, F&& f) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const unsigned w = q == 0 ? t.codes[r].x : q == 1 ? t.codes[r].y : q == 2 ? t.codes[r].z : t.codes[r].w;
-        const plr_mx::v2f v = p == 0   ? plr_mx::decode2<0>(w)
-                              : p == 1 ? plr_mx::decode2<1>(w)
-                              : p == 2 ? plr_mx::decode2<2>(w)
-                                       : plr_mx::decode2<3>(w);
-        f(4 * q + p, r, (double)v[0], (double)v[1]);
-      }
-    }
-  }
+// Values 8 q + 2 p and 8 q + 2 p + 1 of row r, unscaled.
+template <int R>
+__device__ __forceinline__ plr_mx::v2f tile_values(const PackedTile<R>& t, int q, int p, int r) {
+  const unsigned w = q == 0   ? t.codes[r].x
+                     : q == 1 ? t.codes[r].y
+                     : q == 2 ? t.codes[r].z
+                              : t.codes[r].w;
+  return p == 0   ? plr_mx::decode2<0>(w)
+         : p == 1 ? plr_mx::decode2<1>(w)
+         : p == 2 ? plr_mx::decode2<2>(w)
+                  : plr_mx::decode2<3>(w);
 }
 
 // 2^(s - 127) of row r; a block that stands for NaN makes its row's dot product NaN.
@@ -97,26 +99,31 @@ __device__ __forceinline__ double tile_scale(const PackedTile<R>& t, int r) {
   return s == 255u ? __builtin_nan("") : plr_mx::scale_value_f64(s);
 }
 
+constexpr int kPackedR = 4;
+
 // STRIDE: entries between theta's column pairs in LDS, at least `blocks` (fixed, so that a thread's
 // reads share one address).
-template <bool GRAD, bool DROP, int MODE, int STRIDE, int R = kPackedRows>
-__global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a) {
+template <bool GRAD, bool DROP, int MODE, int STRIDE, int SR, int NT, int MINW>
+__global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
+  constexpr int R = kPackedR;
+  static_assert(SR % R == 0, "whole groups of row sets");
   extern __shared__ double sm[];
-  const int tid = threadIdx.x, nt = blockDim.x;
-  const int rows = a.slots * R;  // rows of a tile
-  v2d* const thl = reinterpret_cast<v2d*>(sm);              // [16][STRIDE]: columns 2i, 2i + 1
-  double* const zl = sm + (MODE == kPassAxpy ? 0 : 32 * STRIDE);  // [2][rows][blocks]
-  double* const rl = zl + (size_t)2 * rows * a.blocks;      // [2][rows]
+  const int tid = threadIdx.x;
+  const int max_rows = a.slots * SR;  // rows of a tile
+  const int zpitch = a.blocks | 1; // odd: a row's partials start on another bank than the next one's
+  v2d* const thl = reinterpret_cast<v2d*>(sm);  // [16][STRIDE]: columns 2i, 2i + 1
+  double* const zl = sm + 32 * STRIDE;          // [max_rows][zpitch]
+  double* const rl = zl + (size_t)max_rows * zpitch;  // [max_rows]
+  unsigned* const ml = reinterpret_cast<unsigned*>(rl + max_rows);  // [SR][NT]: dropped values
   const int slot = tid / a.blocks, blk = tid - slot * a.blocks;
   const bool active = slot < a.slots;
-  const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int nwaves = nt / kWave;
+  const int lane = tid & (kWave - 1), wave = tid / kWave;
   double acc[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) acc[i] = 0.;
   if (MODE != kPassAxpy) {
     const v2d* src = reinterpret_cast<const v2d*>(a.theta + (int64_t)a.blk0 * 32);
-    for (int e = tid; e < 16 * a.blocks; e += nt) thl[(e & 15) * STRIDE + (e >> 4)] = src[e];
+    for (int e = tid; e < 16 * a.blocks; e += NT) thl[(e & 15) * STRIDE + (e >> 4)] = src[e];
     __syncthreads();
   }
   plr_mx::MaskGroup group[4];
@@ -126,149 +133,162 @@ __global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a
   }
   RowSums sums;
   const double bias = a.theta_bias ? *a.theta_bias : 0.;
-  const int64_t ntiles = (a.n + rows - 1) / rows;
 
-  // Rows behind the last one, and threads without a block, read a row that is there and count
-  // nothing.
+  // R row sets from set `set` on (behind the last row lie readable zeros: they count nothing).
   const unsigned at_lane = (unsigned)((active ? slot : 0) * a.row_blocks + a.blk0 + blk);
-  auto load = [&](int64_t tile, PackedTile<R>& t) {
-    t.scales = 0;
-    if ((tile + 1) * rows <= a.n) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int64_t at = (tile * rows + r * a.slots) * a.row_blocks;  // the same for all threads
-        t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
-        t.scales |= (unsigned)(a.scales + at)[at_lane] << (8 * r);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        int64_t row = tile * rows + r * a.slots + (active ? slot : 0);
-        row = row < a.n ? row : a.n - 1;
-        const int64_t at = row * a.row_blocks + a.blk0 + blk;
-        t.codes[r] = *reinterpret_cast<const uint4*>(a.codes + at * 16);
-        t.scales |= (unsigned)a.scales[at] << (8 * r);
-      }
-    }
-  };
-  auto drop = [&](int64_t tile, PackedTile<R>& t) {
-    if (!DROP) return;
+  auto load = [&](int64_t set, PackedLoads<R>& t) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const plr_mx::MaskRow mr = plr_mx::mask_row(a.mask, tile * rows + r * a.slots + slot);
-      t.codes[r].x &= plr_mx::keep_nibbles(a.mask, group[0], mr);
-      t.codes[r].y &= plr_mx::keep_nibbles(a.mask, group[1], mr);
-      t.codes[r].z &= plr_mx::keep_nibbles(a.mask, group[2], mr);
-      t.codes[r].w &= plr_mx::keep_nibbles(a.mask, group[3], mr);
+      const int64_t at = (set + r) * a.slots * a.row_blocks;  // the same for all threads
+      t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
+      t.scales[r] = (a.scales + at)[at_lane];
     }
   };
-  auto dot = [&](PackedTile<R>& t, double* z) {
-    double part[R];
+  // Zero what is dropped; marks[r]: bit q + 4 i is value 8 q + i of row r, 1 where dropped.
+  auto drop = [&](int64_t set, PackedTile<R>& t, unsigned (&marks)[R]) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) part[r] = 0.;
-    v2d th;
-    each_value<R>(t, [&](int i, int r, double x0, double x1) {
-      if (r == 0) th = thl[i * STRIDE + blk];
-      part[r] = fma(x0, th.x, part[r]);
-      part[r] = fma(x1, th.y, part[r]);
-      // here, and not all decoded first and summed behind the branch: that takes every register
-      asm volatile("" : "+v"(part[r]));
-    });
-    if (active) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        z[(r * a.slots + slot) * a.blocks + blk] = part[r] * tile_scale(t, r);
+    for (int r = 0; r < R; ++r) {
+      const plr_mx::MaskRow mr = plr_mx::mask_row(a.mask, (set + r) * a.slots + slot);
+      const unsigned m0 = plr_mx::drop_marks(a.mask, group[0], mr);
+      const unsigned m1 = plr_mx::drop_marks(a.mask, group[1], mr);
+      const unsigned m2 = plr_mx::drop_marks(a.mask, group[2], mr);
+      const unsigned m3 = plr_mx::drop_marks(a.mask, group[3], mr);
+      t.codes[r].x &= plr_mx::kept_nibbles(m0);
+      t.codes[r].y &= plr_mx::kept_nibbles(m1);
+      t.codes[r].z &= plr_mx::kept_nibbles(m2);
+      t.codes[r].w &= plr_mx::kept_nibbles(m3);
+      marks[r] = m0 | m1 << 1 | m2 << 2 | m3 << 3;
     }
   };
-  // Row sums and row terms: `per` lanes share a row, a wave takes 64 / per rows at a time, the
-  // waves take turns from tile to tile.
-  auto finish_rows = [&](int64_t tile, const double* z, double* res) {
-    const int per = a.lanes_per_row, step = kWave / per, sub = lane & (per - 1);
-    int first = wave - (int)(tile % nwaves);
-    if (first < 0) first += nwaves;
-    for (int q0 = first * step; q0 < rows; q0 += nwaves * step) {
-      const int q = q0 + lane / per;
-      double s = 0.;
-      if (q < rows) {
-        const double* p = z + (size_t)q * a.blocks;
-#pragma unroll 4
-        for (int b = sub; b < a.blocks; b += per) s += p[b];
-      }
-      for (int m = 1; m < per; m <<= 1) s += __shfl_xor(s, m, kWave);
-      const int64_t row = tile * rows + q;
-      if (q < rows && sub == 0) {
-        double rv = 0.;
-        if (row < a.n) {
-          if (DROP) s *= a.kept;
-          if (MODE == kPassDot) {
-            a.z_buf[row] = a.z_accumulate ? a.z_buf[row] + s : s;
-          } else {
-            double h, l;
-            const double yv = a.y ? a.y[row] : 0.;
-            row_terms(s + bias, yv, a.loss_mode, a.identity_link, h, l);
-            sums.loss += l;
-            rv = h - yv;
-            sums.res += rv;
-            if (a.h_out) store_h(a.h_out + row, h);
-          }
+  auto drop_again = [&](PackedTile<R>& t, int r, unsigned marks) {
+    t.codes[r].x &= plr_mx::kept_nibbles(marks & 0x11111111u);
+    t.codes[r].y &= plr_mx::kept_nibbles(marks >> 1 & 0x11111111u);
+    t.codes[r].z &= plr_mx::kept_nibbles(marks >> 2 & 0x11111111u);
+    t.codes[r].w &= plr_mx::kept_nibbles(marks >> 3 & 0x11111111u);
+  };
+  auto update = [&](const PackedTile<R>& t, const double (&w)[R]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int r = 0; r < R; ++r)  // (eight sums apart between two additions to the same one)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const plr_mx::v2f x = tile_values<R>(t, q, p, r);
+          acc[8 * q + 2 * p] = fma((double)x[0], w[r], acc[8 * q + 2 * p]);
+          acc[8 * q + 2 * p + 1] = fma((double)x[1], w[r], acc[8 * q + 2 * p + 1]);
+          asm volatile("" : "+v"(acc[8 * q + 2 * p]), "+v"(acc[8 * q + 2 * p + 1]));
         }
-        if (GRAD) res[q] = rv;
-      }
-    }
-  };
-  auto update = [&](PackedTile<R>& t, const double* w) {
-    each_value<R>(t, [&](int i, int r, double x0, double x1) {
-      acc[2 * i] = fma(x0, w[r], acc[2 * i]);
-      acc[2 * i + 1] = fma(x1, w[r], acc[2 * i + 1]);
-    });
   };
 
-  const int64_t t0 = blockIdx.x, dt = gridDim.x;
-  if (MODE == kPassAxpy) {
-    PackedTile<R> cur, nxt;
-    if (t0 < ntiles) load(t0, nxt);
-    for (int64_t t = t0; t < ntiles; t += dt) {
-      cur = nxt;
-      if (t + dt < ntiles) load(t + dt, nxt);
-      drop(t, cur);
-      double w[R];
+  // The workgroup's share: consecutive groups of R row sets, shares differing by one at most, in
+  // tiles of up to SR sets.
+  const int64_t share = a.groups / gridDim.x, longer = a.groups - share * gridDim.x;
+  const int64_t first = blockIdx.x * share + min((int64_t)blockIdx.x, longer);
+  const int64_t end = (first + share + ((int64_t)blockIdx.x < longer ? 1 : 0)) * R;
+  PackedLoads<R> nxt;
+  if (first * R < end) load(first * R, nxt);
+  for (int64_t set0 = first * R; set0 < end; set0 += SR) {
+    const int sets = (int)min((int64_t)SR, end - set0);
+    const bool more = set0 + SR < end;
+    if (MODE != kPassAxpy) {
+      for (int s = 0; s < sets; s += R) {
+        PackedTile<R> cur = arrived(nxt);
+        if (s + R < sets) load(set0 + s + R, nxt);
+        else if (GRAD) load(set0, nxt);
+        else if (more) load(set0 + SR, nxt);
+        if (DROP) {
+          unsigned marks[R];
+          drop(set0 + s, cur, marks);
+          if (GRAD) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int64_t row = t * rows + r * a.slots + slot;
-        w[r] = active && row < a.n ? a.res_in[row] * tile_scale(cur, r) : 0.;
-        if (DROP) w[r] *= a.kept;
-      }
-      update(cur, w);
-    }
-  } else {
-    PackedTile<R> prev, cur, nxt;
-    if (t0 < ntiles) load(t0, cur);
-    if (t0 + dt < ntiles) load(t0 + dt, nxt);
-    int par = 0;
-    for (int64_t t = t0; t < ntiles + (GRAD ? dt : 0); t += dt, par ^= 1) {
-      const bool live = t < ntiles;  // (with a gradient the last step only adds the last tile)
-      if (live) {
-        drop(t, cur);
-        dot(cur, zl + (size_t)par * rows * a.blocks);
-      }
-      __syncthreads();
-      if (live) finish_rows(t, zl + (size_t)par * rows * a.blocks, rl + par * rows);
-      if (GRAD) {
-        if (t >= t0 + dt) {
-          forget_decoded(prev);
-          const double* res = rl + (par ^ 1) * rows;
-          double w[R];
+            for (int r = 0; r < R; ++r) ml[(s + r) * NT + tid] = marks[r];
+          }
+        }
+        double part[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[r][0] = part[r][1] = 0.;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const v2d th = thl[i * STRIDE + blk];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            w[r] = active ? res[r * a.slots + slot] * tile_scale(prev, r) : 0.;
-            if (DROP) w[r] *= a.kept;
+            const plr_mx::v2f x = tile_values<R>(cur, i >> 2, i & 3, r);
+            part[r][0] = fma((double)x[0], th.x, part[r][0]);
+            part[r][1] = fma((double)x[1], th.y, part[r][1]);
           }
-          update(prev, w);
+          // here, and not all decoded first and summed behind the branch: that takes every register
+#pragma unroll
+          for (int r = 0; r < R; ++r) asm volatile("" : "+v"(part[r][0]), "+v"(part[r][1]));
         }
-        prev = cur;
+        if (active) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            zl[((s + r) * a.slots + slot) * zpitch + blk] = (part[r][0] + part[r][1]) * tile_scale(cur, r);
+        }
       }
-      cur = nxt;
-      if (t + 2 * dt < ntiles) load(t + 2 * dt, nxt);
+      __syncthreads();
+      const int rows = sets * a.slots;
+      const int per = a.lanes_per_row, sub = tid & (per - 1);
+      for (int q0 = 0; q0 < rows; q0 += NT / per) {
+        const int q = q0 + tid / per;
+        double z = 0.;
+        if (q < rows) {
+          const double* p = zl + q * zpitch;
+#pragma unroll 4
+          for (int b = sub; b < a.blocks; b += per) z += p[b];
+        }
+        for (int m = 1; m < per; m <<= 1) z += __shfl_xor(z, m, kWave);
+        const int64_t row = set0 * a.slots + q;
+        if (q < rows && sub == 0) {
+          double res = 0.;
+          if (row < a.n) {
+            if (DROP) z *= a.kept;
+            if (MODE == kPassDot) {
+              a.z_buf[row] = a.z_accumulate ? a.z_buf[row] + z : z;
+            } else {
+              double h, l;
+              const double yv = a.y ? a.y[row] : 0.;
+              row_terms(z + bias, yv, a.loss_mode, a.identity_link, h, l);
+              sums.loss += l;
+              res = h - yv;
+              sums.res += res;
+              if (a.h_out) store_h(a.h_out + row, h);
+            }
+          }
+          if (GRAD) rl[q] = res;
+        }
+      }
+      __syncthreads();
+    }
+    if (GRAD) {
+#pragma unroll 1
+      for (int s = 0; s < sets; s += R) {
+        PackedTile<R> cur = arrived(nxt);
+        if (s + R < sets) load(set0 + s + R, nxt);
+        else if (more) load(set0 + SR, nxt);
+        double w[R];
+        if (MODE == kPassAxpy) {
+          if (DROP) {
+            unsigned marks[R];
+            drop(set0 + s, cur, marks);
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int64_t row = (set0 + s + r) * a.slots + slot;
+            w[r] = active && row < a.n ? a.res_in[row] * tile_scale(cur, r) : 0.;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (DROP) drop_again(cur, r, ml[(s + r) * NT + tid]);
+            w[r] = active ? rl[(s + r) * a.slots + slot] * tile_scale(cur, r) : 0.;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (DROP) w[r] *= a.kept;
+        update(cur, w);
+      }
     }
   }
   if (GRAD) {
@@ -281,7 +301,7 @@ __global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a
         for (int i = 0; i < 8; ++i) sm[tid * 8 + i] = acc[8 * q + i];
       }
       __syncthreads();
-      for (int e = tid; e < a.blocks * 8; e += nt) {
+      for (int e = tid; e < a.blocks * 8; e += NT) {
         const int b = e >> 3, i = e & 7;
         double g = 0.;
         for (int s = 0; s < a.slots; ++s) g += sm[(s * a.blocks + b) * 8 + i];
@@ -290,25 +310,7 @@ __global__ __launch_bounds__(kPackedMaxThreads, 2) void packed_pass(PackedArgs a
       __syncthreads();
     }
   }
-  if (MODE == kPassFused) {
-    // the waves' loss and residual sums, in wave order
-    __shared__ double lx[kPackedMaxThreads / kWave], rx[kPackedMaxThreads / kWave];
-    const double wl = wave_sum(sums.loss), wr = wave_sum(sums.res);
-    if (lane == 0) {
-      lx[wave] = wl;
-      rx[wave] = wr;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      double l = 0., r = 0.;
-      for (int w = 0; w < nwaves; ++w) {
-        l += lx[w];
-        r += rx[w];
-      }
-      a.part_loss[blockIdx.x] = l;
-      if (a.part_res) a.part_res[blockIdx.x] = r;
-    }
-  }
+  if (MODE == kPassFused) emit_row_sums<NT / kWave>(sums, lane, wave, a.part_loss, a.part_res);
 }
 
 }  // namespace plr
