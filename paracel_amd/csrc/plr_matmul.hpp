@@ -9,6 +9,7 @@
 
 namespace plr_mx {
 
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -21,86 +22,266 @@ struct MatmulArgs {
   int64_t ldc;
   float alpha;
   float kept;  // dropout: the factor of what is kept
+  int wide_store;  // rows of c start on 16-byte boundaries
   Mask mask;
 };
 
-// 16 bytes = one block of 32 values, in the low half of the instruction's operand.
-__device__ __forceinline__ v8i operand(const uint8_t* p) {
-  const int4 w = *reinterpret_cast<const int4*>(p);
-  return v8i{w.x, w.y, w.z, w.w, 0, 0, 0, 0};
+// One block of 32 values, in the low half of the instruction's operand.
+__device__ __forceinline__ v8i operand(v4i w) {
+  return __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
 }
 
+template <int SEL>
+__device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(a), operand(b), c, 4, 4, SEL, sa,
+                                                          SEL, sb);
+}
+
+// ------------------------------------------------------------------- epilogue
 template <typename T>
-__device__ __forceinline__ T narrow(float v) {
-  return (T)v;
-}
+struct alignas(16) Out8 {
+  T v[8];
+};
 
-// Simple form: a wave owns 32 x 32 of C, four waves 64 x 64.  For the 16 x 16 x 128 instruction
-// lane l holds row l % 16 and block l / 16 of the 128 values: 16 consecutive bytes of a code row
-// and one scale byte.  Rows past the end are read as the last row and not stored.
+// Columns j .. j + 7 of row i (j a multiple of 8): factor, dropout, one rounding, store.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(256) void matmul_simple(MatmulArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i0 = (int64_t)blockIdx.y * 64 + (wave >> 1) * 32;
-  const int64_t j0 = (int64_t)blockIdx.x * 64 + (wave & 1) * 32;
-  const int r16 = lane & 15, q = lane >> 4;
-  const uint8_t *pa[2], *pb[2], *qa[2], *qb[2];
+__device__ __forceinline__ void store8(const MatmulArgs& p, int64_t i, int64_t j, v4f lo, v4f hi) {
+  if (i >= p.m || j >= p.n) return;
+  const unsigned drops = DROP ? drop_marks(p.mask, i, (unsigned)(j >> 3)) : 0u;
+  Out8<T> o;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int64_t i = min(i0 + 16 * t + r16, p.m - 1), j = min(j0 + 16 * t + r16, p.n - 1);
-    pa[t] = p.a + i * p.lda + q * 16;
-    pb[t] = p.b + j * p.ldb + q * 16;
-    qa[t] = p.sa + i * p.ldsa + q;
-    qb[t] = p.sb + j * p.ldsb + q;
+  for (int e = 0; e < 8; ++e) {
+    float v = p.alpha * (e < 4 ? lo[e & 3] : hi[e & 3]);
+    if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * p.kept;
+    o.v[e] = (T)v;
   }
-  v4f acc[2][2] = {};
-  for (int k = 0; k < p.chunks; ++k) {
-    v8i a[2], b[2];
-    int sa[2], sb[2];
+  T* c = static_cast<T*>(p.c) + i * p.ldc + j;
+  if (p.wide_store && j + 8 <= p.n) {
+    *reinterpret_cast<Out8<T>*>(c) = o;
+  } else {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      a[t] = operand(pa[t] + (int64_t)k * 64);
-      b[t] = operand(pb[t] + (int64_t)k * 64);
-      sa[t] = qa[t][(int64_t)k * 4];
-      sb[t] = qb[t][(int64_t)k * 4];
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        acc[x][y] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[x], b[y], acc[x][y], 4, 4, 0,
-                                                                     sa[x], 0, sb[y]);
+    for (int e = 0; e < 8; ++e)
+      if (j + e < p.n) c[e] = o.v[e];
   }
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t i = i0 + 16 * x + q * 4 + e, j = j0 + 16 * y + r16;
-        if (i >= p.m || j >= p.n) continue;
-        float v = p.alpha * acc[x][y][e];
-        if (DROP) v = (drop_marks(p.mask, i, (unsigned)(j >> 3)) >> 4 * (j & 7) & 1) ? 0.f : v * p.kept;
-        static_cast<T*>(p.c)[i * p.ldc + j] = narrow<T>(v);
-      }
 }
 
-template <typename T>
-inline void launch_simple(const MatmulArgs& a, bool drop, dim3 grid, hipStream_t st) {
-  auto f = drop ? matmul_simple<T, true> : matmul_simple<T, false>;
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, st, a);
+// Workgroups that follow each other go to the 8 XCDs in turn: give every XCD a run of tiles, and
+// lay a run out in groups of 8 tile rows, so that the tiles an XCD works on at a time share their
+// rows of A and B in its L2.
+__device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned tiles_n, unsigned& tm,
+                                        unsigned& tn) {
+  const unsigned total = tiles_m * tiles_n, per = total / 8, rem = total % 8;
+  const unsigned xcd = id % 8;
+  const unsigned t = xcd * per + min(xcd, rem) + id / 8;
+  const unsigned group = t / (8 * tiles_n), first = group * 8;
+  const unsigned height = min(8u, tiles_m - first), in = t - group * 8 * tiles_n;
+  tm = first + in % height;
+  tn = in / height;
+}
+
+// ------------------------------------------------------------------- large products
+// A workgroup owns BM x BN of C, a wave WM x WN, in 16 x 16 x 128 instructions: lane l holds block
+// l / 16 (32 values, 16 bytes, one scale byte) of row l % 16.  The rows of B go in as the
+// instruction's first operand, so that a lane's four sums are four columns of one row of C, and a
+// pair of 16-row pieces is dealt out so that they are eight: 16 consecutive bytes of bfloat16.
+//
+// 128 values of k are a step.  Codes pass through a ring of four stages in LDS, filled by
+// asynchronous loads three steps ahead; a step's pieces of B and its first two of A were read
+// from LDS during the step before, the other pieces of A two ahead of their use.  Within a row's
+// 64 bytes of a stage the four blocks are permuted by the row number, so that the 16 rows a wave
+// reads at once lie on different banks.
+//
+// Scales go the same way, 16 bytes per row and group of four steps, in a ring of three groups; a
+// lane picks its block's four bytes into one word once per group, and the instruction selects the
+// byte of its step.
+// The asynchronous loads are written as instructions: the compiler holds every later read of LDS
+// until all of them have landed, whichever stage it reads.  They have no register results; the
+// waits are the step's own.
+__device__ __forceinline__ void copy_to_lds(const uint8_t* base, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+__device__ __forceinline__ void copy_word_to_lds(const uint8_t* src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               ::"s"(lds), "v"(src) : "memory");
+}
+
+template <typename T, bool DROP, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(MatmulArgs p, unsigned tiles_m,
+                                                                              unsigned tiles_n) {
+  constexpr int NT = 64 * (BM / WM) * (BN / WN);
+  constexpr int FM = WM / 16, FN = WN / 16;        // 16-row pieces of a wave
+  constexpr int LA = BM * 4 / NT, LB = BN * 4 / NT;  // asynchronous loads per thread and step
+  constexpr int ROWS = BM + BN;
+  static_assert(ROWS == NT, "four words of scales per row and group, one load per thread and step");
+  static_assert(LA + LB <= FM && FN <= FM && FM >= 4, "a step's loads and reads fit its rows of instructions");
+  __shared__ v4i stage[4][ROWS * 4];
+  __shared__ v4i scale[3][ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const int kc = p.chunks;
+
+  // what this thread loads: row tid / 4 (+ NT / 4 * i) of the tile, block (tid % 4) ^ (row's permutation)
+  const int lr = tid >> 2;
+  const int ka = (tid & 3) ^ ((lr >> 1) & 3), kb = (tid & 3) ^ (((lr >> 1) & 1) | ((lr >> 2) & 2));
+  const uint8_t* const abase = p.a + m0 * p.lda;
+  const uint8_t* const bbase = p.b + n0 * p.ldb;
+  unsigned aoff[LA], boff[LB];
+#pragma unroll
+  for (int i = 0; i < LA; ++i)
+    aoff[i] = (unsigned)(min((int64_t)(lr + NT / 4 * i), p.m - 1 - m0) * p.lda + ka * 16);
+#pragma unroll
+  for (int i = 0; i < LB; ++i)
+    boff[i] = (unsigned)(min((int64_t)(lr + NT / 4 * i), p.n - 1 - n0) * p.ldb + kb * 16);
+  const unsigned lds0 = lds_address(&stage[0][0]) + (unsigned)wave * 1024u;
+  // load i of the LA + LB that bring step k's codes into stage st
+  auto fill = [&](int st, int k, int i) {
+    const int64_t at = (int64_t)min(k, kc - 1) * 64;
+    const unsigned to = lds0 + (unsigned)(st * ROWS * 64 + i * NT * 16);
+    if (i < LA) copy_to_lds(abase + at, aoff[i], to);
+    else copy_to_lds(bbase + at, boff[i - LA], to);
+  };
+  // a group's scales: load i brings the words of steps k .. k + 3 (the last step's again behind
+  // the end) of rows ROWS / 4 * i + tid / 4 into ring place `to`
+  const uint8_t* srow[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = ROWS / 4 * i + (tid >> 2);
+    srow[i] = r < BM ? p.sa + min(m0 + r, p.m - 1) * p.ldsa : p.sb + min(n0 + r - BM, p.n - 1) * p.ldsb;
+  }
+  const unsigned lds1 = lds_address(&scale[0][0]) + (unsigned)wave * 256u;
+  auto fill_scales = [&](int to, int k, int i) {
+    copy_word_to_lds(srow[i] + (int64_t)min(k + (tid & 3), kc - 1) * 4,
+                     lds1 + (unsigned)(to * ROWS * 16 + i * ROWS * 4));
+  };
+
+  // rows of the pieces: A straight, B dealt out by eights
+  const int arow = wm + r16;
+  const int brow = wn + (r16 >> 2) * 8 + (r16 & 3);
+  const int apos = arow * 4 + (q ^ ((arow >> 1) & 3));  // + 64 per piece: 16 rows on, same permutation
+  auto bpos = [&](int f) {
+    const int r = brow + (f >> 1) * 32 + (f & 1) * 4;
+    return (BM + r) * 4 + (q ^ (((r >> 1) & 1) | ((r >> 2) & 2)));
+  };
+  auto read_a = [&](int st, int f) { return stage[st][apos + 64 * f]; };
+  auto read_b = [&](int st, int f) { return stage[st][bpos(f)]; };
+  // bytes q of a row's four words, in one word
+  const unsigned pick0 = 0x0c0c0400u + 0x0101u * q, pick1 = 0x04000c0cu + 0x01010000u * q;
+  auto scales_of = [&](int from, int row) {
+    const v4i w = scale[from][row];
+    return (int)(__builtin_amdgcn_perm(w[1], w[0], pick0) | __builtin_amdgcn_perm(w[3], w[2], pick1));
+  };
+  auto scale_a = [&](int from, int f) { return scales_of(from, arow + 16 * f); };
+  auto scale_b = [&](int from, int f) { return scales_of(from, BM + brow + (f >> 1) * 32 + (f & 1) * 4); };
+  v4i fa[FM], fb[FN], na[2], nb[FN];  // pieces of this step and of the next
+  int xa[FM], xb[FN], ya[FM], yb[FN];
+  v4f acc[FM][FN];
+#pragma unroll
+  for (int x = 0; x < FM; ++x)
+#pragma unroll
+    for (int y = 0; y < FN; ++y) acc[x][y] = v4f{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    fill_scales(0, 0, i);
+    fill_scales(1, 4, i);
+  }
+#pragma unroll
+  for (int st = 0; st < 3; ++st)
+#pragma unroll
+    for (int i = 0; i < LA + LB; ++i) fill(st, st, i);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int f = 0; f < FN; ++f) {
+    fb[f] = read_b(0, f);
+    xb[f] = scale_b(0, f);
+  }
+#pragma unroll
+  for (int f = 0; f < FM; ++f) xa[f] = scale_a(0, f);
+  fa[0] = read_a(0, 0);
+  fa[1] = read_a(0, 1);
+
+  // Step J of a group of four, k the group's first.  The codes of step k + J + 1 have arrived when
+  // at most the loads of the step after it are under way; those of step k + J + 3 leave for the
+  // stage that step k + J - 1 was read from, and a quarter of the scales of two groups on.  The
+  // next group's scales are read in step 3.
+#define PLR_STEP(J)                                                                              \
+  {                                                                                              \
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB + 1) : "memory");                           \
+    __builtin_amdgcn_s_barrier();                                                                \
+    __builtin_amdgcn_sched_barrier(0);                                                           \
+    _Pragma("unroll") for (int x = 0; x < FM; ++x) {                                             \
+      if (x + 2 < FM) fa[x + 2] = read_a(J, x + 2);                                              \
+      if (x < LA + LB) fill((J + 3) & 3, k + J + 3, x);                                          \
+      if (x == FM - 1) fill_scales(place == 0 ? 2 : place - 1, k + 8, J);                        \
+      if (x >= FM - FN) nb[x - (FM - FN)] = read_b((J + 1) & 3, x - (FM - FN));                  \
+      if (x >= FM - 2) na[x - (FM - 2)] = read_a((J + 1) & 3, x - (FM - 2));                     \
+      if (J == 3) {                                                                              \
+        ya[x] = scale_a(place == 2 ? 0 : place + 1, x);                                          \
+        if (x < FN) yb[x] = scale_b(place == 2 ? 0 : place + 1, x);                              \
+      }                                                                                          \
+      _Pragma("unroll") for (int y = 0; y < FN; ++y) acc[x][y] =                                 \
+          mfma<J>(fb[y], fa[x], acc[x][y], xb[y], xa[x]);                                        \
+      __builtin_amdgcn_sched_barrier(0);                                                         \
+    }                                                                                            \
+    _Pragma("unroll") for (int f = 0; f < FN; ++f) fb[f] = nb[f];                                \
+    fa[0] = na[0];                                                                               \
+    fa[1] = na[1];                                                                               \
+    if (J == 3) {                                                                                \
+      _Pragma("unroll") for (int f = 0; f < FM; ++f) xa[f] = ya[f];                              \
+      _Pragma("unroll") for (int f = 0; f < FN; ++f) xb[f] = yb[f];                              \
+      place = place == 2 ? 0 : place + 1;                                                        \
+    }                                                                                            \
+  }
+  int k = 0, place = 0;  // place: of the group's scales in the ring
+  for (; k + 4 <= kc; k += 4) {
+    PLR_STEP(0)
+    PLR_STEP(1)
+    PLR_STEP(2)
+    PLR_STEP(3)
+  }
+  if (k < kc) PLR_STEP(0)
+  if (k + 1 < kc) PLR_STEP(1)
+  if (k + 2 < kc) PLR_STEP(2)
+#undef PLR_STEP
+  // the loads of the steps behind the last one still write to LDS
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < FM; ++x)
+#pragma unroll
+    for (int y = 0; y < FN; y += 2)
+      store8<T, DROP>(p, m0 + wm + 16 * x + r16, n0 + wn + (y >> 1) * 32 + q * 8, acc[x][y], acc[x][y + 1]);
+}
+
+// ------------------------------------------------------------------- launch
+template <int BM, int BN, int WM, int WN>
+inline bool launch_tiles(const MatmulArgs& a, int type, bool drop, hipStream_t st) {
+  const int64_t tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
+  if (tm > 0x7fffff / tn) return false;
+  auto f = type == 0 ? (drop ? matmul_tiles<float, true, BM, BN, WM, WN> : matmul_tiles<float, false, BM, BN, WM, WN>)
+           : type == 1 ? (drop ? matmul_tiles<__bf16, true, BM, BN, WM, WN>
+                               : matmul_tiles<__bf16, false, BM, BN, WM, WN>)
+                       : (drop ? matmul_tiles<_Float16, true, BM, BN, WM, WN>
+                               : matmul_tiles<_Float16, false, BM, BN, WM, WN>);
+  hipLaunchKernelGGL(f, dim3((unsigned)(tm * tn)), dim3(64 * (BM / WM) * (BN / WN)), 0, st, a, (unsigned)tm,
+                     (unsigned)tn);
+  return true;
 }
 
 // type: 0 float, 1 bfloat16, 2 half.  False when the grid would not fit one launch.
 inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hipStream_t st) {
-  (void)cus;
-  const int64_t gx = (a.n + 63) / 64, gy = (a.m + 63) / 64;
-  if (gy > 65535 || gx > 0x7fffffff) return false;
-  const dim3 grid((unsigned)gx, (unsigned)gy);
-  if (type == 0) launch_simple<float>(a, drop, grid, st);
-  else if (type == 1) launch_simple<__bf16>(a, drop, grid, st);
-  else launch_simple<_Float16>(a, drop, grid, st);
-  return true;
+  const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+  if (big >= cus / 2) return launch_tiles<256, 256, 128, 64>(a, type, drop, st);
+  return launch_tiles<128, 128, 64, 64>(a, type, drop, st);
 }
 
 }  // namespace plr_mx

@@ -645,8 +645,10 @@ int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64
   if (size == 0 || type == PLR_F64)
     return c.bad(PLR_ERR_INVALID, "the result is PLR_F32, PLR_BF16 or PLR_F16");
   if (m < 0 || n < 0 || k < 1) return c.bad(PLR_ERR_INVALID, "need m >= 0, n >= 0 and k >= 1");
-  if (m > (int64_t)1 << 31 || n > (int64_t)1 << 31 || k > (int64_t)1 << 31)
-    return c.bad(PLR_ERR_INVALID, "m, n and k must be at most 2^31");
+  if (m > (int64_t)1 << 31 || n > (int64_t)1 << 31)
+    return c.bad(PLR_ERR_INVALID, "m and n must be at most 2^31");
+  if (k > (int64_t)1 << 24 || lda > (int64_t)1 << 23 || ldb > (int64_t)1 << 23)
+    return c.bad(PLR_ERR_INVALID, "k must be at most 2^24 and a code pitch 2^23 bytes");
   if (lda % 64 != 0 || ldb % 64 != 0 || lda < plr_mxfp_code_pitch(k) || ldb < plr_mxfp_code_pitch(k))
     return c.bad(PLR_ERR_INVALID, "code pitches must be multiples of 64 and at least plr_mxfp_code_pitch(k)");
   if (ldsa % 4 != 0 || ldsb % 4 != 0 || ldsa < plr_mxfp_scale_pitch(k) || ldsb < plr_mxfp_scale_pitch(k))
@@ -683,6 +685,7 @@ int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64
   a.ldc = ldc;
   a.alpha = (float)alpha;
   a.kept = (float)scale;
+  a.wide_store = aligned(dc, 16) && ldc * (int64_t)size % 16 == 0;
   rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || m == 0 || n == 0) return rc;
   const bool dr = drop != nullptr && a.mask.threshold > 0;
