@@ -43,10 +43,9 @@ struct alignas(16) Out8 {
   T v[8];
 };
 
-// Columns j .. j + 7 of row i (j a multiple of 8): factor, dropout, one rounding, store.
+// Columns j .. j + 7 of row i (j a multiple of 8): factor, dropout, one rounding.
 template <typename T, bool DROP>
-__device__ __forceinline__ void store8(const MatmulArgs& p, int64_t i, int64_t j, v4f lo, v4f hi) {
-  if (i >= p.m || j >= p.n) return;
+__device__ __forceinline__ Out8<T> finish8(const MatmulArgs& p, int64_t i, int64_t j, v4f lo, v4f hi) {
   const unsigned drops = DROP ? drop_marks(p.mask, i, (unsigned)(j >> 3)) : 0u;
   Out8<T> o;
 #pragma unroll
@@ -55,10 +54,37 @@ __device__ __forceinline__ void store8(const MatmulArgs& p, int64_t i, int64_t j
     if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * p.kept;
     o.v[e] = (T)v;
   }
-  T* c = static_cast<T*>(p.c) + i * p.ldc + j;
-  if (p.wide_store && j + 8 <= p.n) {
-    *reinterpret_cast<Out8<T>*>(c) = o;
-  } else {
+  return o;
+}
+
+// A wave's 16 x (16 FN) piece of C, rows i0 .., columns j0 ..; lane (r16, q) holds columns
+// 32 (y / 2) + 8 q .. + 7 of row r16 in acc[y], acc[y + 1] (y even).  Tiles that lie inside C are
+// stored as they are held; those at its edge, or on rows without alignment, go through 1 KB of LDS
+// per wave and 32 columns, so that the code with the comparisons is there once and not for every
+// register.
+template <typename T, bool DROP, int FN>
+__device__ __forceinline__ void store_piece(const MatmulArgs& p, int64_t i0, int64_t j0, const v4f* acc, int r16,
+                                            int q) {
+  T* c = static_cast<T*>(p.c) + (i0 + r16) * p.ldc + j0 + q * 8;
+#pragma unroll
+  for (int y = 0; y < FN; y += 2)
+    *reinterpret_cast<Out8<T>*>(c + y * 16) =
+        finish8<T, DROP>(p, i0 + r16, j0 + y * 16 + q * 8, acc[y], acc[y + 1]);
+}
+template <typename T, bool DROP, int FN>
+__device__ __forceinline__ void store_edge_piece(const MatmulArgs& p, int64_t i0, int64_t j0, const v4f* acc,
+                                                 int r16, int q, v4f* lds) {
+  // lds: FN / 2 x 64 lanes x 2
+#pragma unroll
+  for (int y = 0; y < FN; ++y) lds[((y >> 1) * 64 + q * 16 + r16) * 2 + (y & 1)] = acc[y];
+  const int64_t i = i0 + r16;
+#pragma unroll 1
+  for (int y = 0; y < FN / 2; ++y) {
+    const int64_t j = j0 + y * 32 + q * 8;
+    if (i >= p.m || j >= p.n) continue;
+    const v4f* from = lds + (y * 64 + q * 16 + r16) * 2;
+    const Out8<T> o = finish8<T, DROP>(p, i, j, from[0], from[1]);
+    T* c = static_cast<T*>(p.c) + i * p.ldc + j;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (j + e < p.n) c[e] = o.v[e];
@@ -255,11 +281,17 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
 #undef PLR_STEP
   // the loads of the steps behind the last one still write to LDS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (p.wide_store && m0 + BM <= p.m && n0 + BN <= p.n) {
 #pragma unroll
-  for (int x = 0; x < FM; ++x)
+    for (int x = 0; x < FM; ++x)
+      store_piece<T, DROP, FN>(p, m0 + wm + 16 * x, n0 + wn, acc[x], r16, q);
+  } else {
+    __builtin_amdgcn_s_barrier();  // every wave's loads have landed
+    v4f* const mine = reinterpret_cast<v4f*>(&stage[0][0]) + wave * (FN / 2 * 128);
 #pragma unroll
-    for (int y = 0; y < FN; y += 2)
-      store8<T, DROP>(p, m0 + wm + 16 * x + r16, n0 + wn + (y >> 1) * 32 + q * 8, acc[x][y], acc[x][y + 1]);
+    for (int x = 0; x < FM; ++x)
+      store_edge_piece<T, DROP, FN>(p, m0 + wm + 16 * x, n0 + wn, acc[x], r16, q, mine);
+  }
 }
 
 // ------------------------------------------------------------------- launch
