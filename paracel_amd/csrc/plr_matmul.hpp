@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "plr_mxfp.hpp"
 
 namespace plr_mx {
@@ -294,6 +296,132 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
   }
 }
 
+// ------------------------------------------------------------------- few rows on one side
+// At most 64 rows of the one operand ("few") against many of the other: bound by the bytes of the
+// many, which are read once, straight into the instruction's operands.  A workgroup owns 16 FX rows
+// of the many; its W waves divide k, and their sums meet in LDS in wave order.  Codes of four
+// chunks are requested at once: 256 consecutive bytes of a row.
+struct FewArgs {
+  MatmulArgs p;
+  const uint8_t *x, *y, *sx, *sy;  // many, few
+  int64_t ldx, ldy, ldsx, ldsy;
+  int64_t rows;  // of x
+  int few;       // rows of y
+};
+
+struct alignas(4) Words4 {
+  int w[4];
+};
+
+template <typename T, bool DROP, int FY, int FX, int W, bool SWAP>
+__global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
+  __shared__ v4f part[W > 1 ? W - 1 : 1][FX * FY][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int64_t x0 = (int64_t)blockIdx.x * (16 * FX);
+  const uint8_t *px[FX], *qx[FX], *py[FY], *qy[FY];
+#pragma unroll
+  for (int f = 0; f < FX; ++f) {
+    const int64_t r = min(x0 + 16 * f + r16, a.rows - 1);
+    px[f] = a.x + r * a.ldx + q * 16;
+    qx[f] = a.sx + r * a.ldsx;
+  }
+#pragma unroll
+  for (int f = 0; f < FY; ++f) {
+    const int r = min(16 * f + r16, a.few - 1);
+    py[f] = a.y + (int64_t)r * a.ldy + q * 16;
+    qy[f] = a.sy + (int64_t)r * a.ldsy;
+  }
+  v4f acc[FX][FY];
+#pragma unroll
+  for (int x = 0; x < FX; ++x)
+#pragma unroll
+    for (int y = 0; y < FY; ++y) acc[x][y] = v4f{0.f, 0.f, 0.f, 0.f};
+  // this wave's chunks: whole groups of four, shares differing by one group at most
+  const int groups = (a.p.chunks + 3) / 4;
+  const int k0 = (int)((int64_t)groups * wave / W) * 4;
+  const int k1 = min((int)((int64_t)groups * (wave + 1) / W) * 4, a.p.chunks);
+  // bytes q of a row's four scale words, in one word
+  const unsigned pick0 = 0x0c0c0400u + 0x0101u * q, pick1 = 0x04000c0cu + 0x01010000u * q;
+  auto scales = [&](const uint8_t* s, int k) {
+    const Words4 w = *reinterpret_cast<const Words4*>(s + (int64_t)k * 4);
+    return (int)(__builtin_amdgcn_perm(w.w[1], w.w[0], pick0) | __builtin_amdgcn_perm(w.w[3], w.w[2], pick1));
+  };
+  auto codes = [&](const uint8_t* s, int k) { return *reinterpret_cast<const v4i*>(s + (int64_t)k * 64); };
+  int k = k0;
+  for (; k + 4 <= k1; k += 4) {
+    v4i cx[4][FX], cy[4][FY];
+    int sx[FX], sy[FY];
+#pragma unroll
+    for (int f = 0; f < FX; ++f) sx[f] = scales(qx[f], k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int f = 0; f < FX; ++f) cx[j][f] = codes(px[f], k + j);
+#pragma unroll
+    for (int f = 0; f < FY; ++f) sy[f] = scales(qy[f], k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int f = 0; f < FY; ++f) cy[j][f] = codes(py[f], k + j);
+#pragma unroll
+    for (int x = 0; x < FX; ++x)
+#pragma unroll
+      for (int y = 0; y < FY; ++y) {
+        acc[x][y] = mfma<0>(cx[0][x], cy[0][y], acc[x][y], sx[x], sy[y]);
+        acc[x][y] = mfma<1>(cx[1][x], cy[1][y], acc[x][y], sx[x], sy[y]);
+        acc[x][y] = mfma<2>(cx[2][x], cy[2][y], acc[x][y], sx[x], sy[y]);
+        acc[x][y] = mfma<3>(cx[3][x], cy[3][y], acc[x][y], sx[x], sy[y]);
+      }
+  }
+  for (; k < k1; ++k) {
+#pragma unroll
+    for (int x = 0; x < FX; ++x)
+#pragma unroll
+      for (int y = 0; y < FY; ++y)
+        acc[x][y] = mfma<0>(codes(px[x], k), codes(py[y], k), acc[x][y], qx[x][(int64_t)k * 4 + q],
+                            qy[y][(int64_t)k * 4 + q]);
+  }
+  if (W > 1) {
+    if (wave > 0) {
+#pragma unroll
+      for (int x = 0; x < FX; ++x)
+#pragma unroll
+        for (int y = 0; y < FY; ++y) part[wave - 1][x * FY + y][lane] = acc[x][y];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int x = 0; x < FX; ++x)
+#pragma unroll
+      for (int y = 0; y < FY; ++y)
+#pragma unroll
+        for (int w = 0; w < W - 1; ++w) acc[x][y] += part[w][x * FY + y][lane];
+  }
+  // lane (r16, q): rows x0 + 16 x + 4 q .. + 3 of the many, row 16 y + r16 of the few
+#pragma unroll
+  for (int x = 0; x < FX; ++x)
+#pragma unroll
+    for (int y = 0; y < FY; ++y) {
+      const int64_t xr = x0 + 16 * x + 4 * q, yr = 16 * y + r16;
+      if (xr >= a.rows || yr >= a.few) continue;
+      unsigned drops = 0;
+      if (DROP && !SWAP) drops = drop_marks(a.p.mask, yr, (unsigned)(xr >> 3)) >> 4 * (xr & 7);
+      T out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = a.p.alpha * acc[x][y][e];
+        if (DROP && SWAP) drops = drop_marks(a.p.mask, xr + e, (unsigned)(yr >> 3)) >> 4 * (yr & 7) << 4 * e;
+        if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * a.p.kept;
+        out[e] = (T)v;
+      }
+      T* c = static_cast<T*>(a.p.c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (xr + e < a.rows) c[SWAP ? (xr + e) * a.p.ldc + yr : yr * a.p.ldc + xr + e] = out[e];
+    }
+}
+
 // ------------------------------------------------------------------- launch
 template <int BM, int BN, int WM, int WN>
 inline bool launch_tiles(const MatmulArgs& a, int type, bool drop, hipStream_t st) {
@@ -309,8 +437,61 @@ inline bool launch_tiles(const MatmulArgs& a, int type, bool drop, hipStream_t s
   return true;
 }
 
+template <typename T, bool DROP, int FY, int FX, int W>
+inline void launch_few_as(const FewArgs& a, bool swap, hipStream_t st) {
+  auto f = swap ? matmul_few<T, DROP, FY, FX, W, true> : matmul_few<T, DROP, FY, FX, W, false>;
+  hipLaunchKernelGGL(f, dim3((unsigned)((a.rows + 16 * FX - 1) / (16 * FX))), dim3(64 * W), 0, st, a);
+}
+template <typename T, bool DROP>
+inline void launch_few(const FewArgs& a, bool swap, int cus, hipStream_t st) {
+  const int fy = (a.few + 15) / 16;
+  const int64_t pieces = (a.rows + 15) / 16;
+  if (fy == 1) {
+    // few workgroups: more waves of each share k (1 x 256 x 16384 9.7 us)
+    if (pieces < (int64_t)cus * 4 && a.p.chunks >= 16) launch_few_as<T, DROP, 1, 1, 8>(a, swap, st);
+    else launch_few_as<T, DROP, 1, 1, 4>(a, swap, st);
+  } else if (pieces >= (int64_t)cus * 2) {
+    // two pieces of the many share what is loaded of the few, where that leaves a workgroup per
+    // compute unit (48 x 16384 x 8192: 29 us, with one piece 42; 32 x 4096 x 4096: 9.2 and 7.8)
+    if (fy == 2) launch_few_as<T, DROP, 2, 2, 4>(a, swap, st);
+    else if (fy == 3) launch_few_as<T, DROP, 3, 2, 4>(a, swap, st);
+    else launch_few_as<T, DROP, 4, 2, 4>(a, swap, st);
+  } else {
+    if (fy == 2) launch_few_as<T, DROP, 2, 1, 4>(a, swap, st);
+    else if (fy == 3) launch_few_as<T, DROP, 3, 1, 4>(a, swap, st);
+    else launch_few_as<T, DROP, 4, 1, 4>(a, swap, st);
+  }
+}
+// Up to 32 rows always; up to 64 where tiles of 128 would leave half the device idle (48 x 16384 x
+// 8192: tiles 27 us, this 29; 33 x 9000 x 4100: 16 and 12).
+inline bool few_rows(const MatmulArgs& p, int cus) {
+  const int64_t few = std::min(p.m, p.n), many = std::max(p.m, p.n);
+  return few <= 32 || (few <= 64 && many < (int64_t)cus * 64);
+}
+inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, hipStream_t st) {
+  const bool swap = p.n < p.m;  // few columns of C: the rows of A are the many
+  FewArgs a;
+  a.p = p;
+  a.x = swap ? p.a : p.b;
+  a.y = swap ? p.b : p.a;
+  a.sx = swap ? p.sa : p.sb;
+  a.sy = swap ? p.sb : p.sa;
+  a.ldx = swap ? p.lda : p.ldb;
+  a.ldy = swap ? p.ldb : p.lda;
+  a.ldsx = swap ? p.ldsa : p.ldsb;
+  a.ldsy = swap ? p.ldsb : p.ldsa;
+  a.rows = swap ? p.m : p.n;
+  a.few = (int)(swap ? p.n : p.m);
+  if (a.rows > (int64_t)0x7fffff * 16) return false;
+  if (type == 0) drop ? launch_few<float, true>(a, swap, cus, st) : launch_few<float, false>(a, swap, cus, st);
+  else if (type == 1) drop ? launch_few<__bf16, true>(a, swap, cus, st) : launch_few<__bf16, false>(a, swap, cus, st);
+  else drop ? launch_few<_Float16, true>(a, swap, cus, st) : launch_few<_Float16, false>(a, swap, cus, st);
+  return true;
+}
+
 // type: 0 float, 1 bfloat16, 2 half.  False when the grid would not fit one launch.
 inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hipStream_t st) {
+  if (few_rows(a, cus)) return launch_few_rows(a, type, drop, cus, st);
   const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
   if (big >= cus / 2) return launch_tiles<256, 256, 128, 64>(a, type, drop, st);
   return launch_tiles<128, 128, 64, 64>(a, type, drop, st);

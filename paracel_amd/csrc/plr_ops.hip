@@ -647,8 +647,9 @@ int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64
   if (m < 0 || n < 0 || k < 1) return c.bad(PLR_ERR_INVALID, "need m >= 0, n >= 0 and k >= 1");
   if (m > (int64_t)1 << 31 || n > (int64_t)1 << 31)
     return c.bad(PLR_ERR_INVALID, "m and n must be at most 2^31");
-  if (k > (int64_t)1 << 24 || lda > (int64_t)1 << 23 || ldb > (int64_t)1 << 23)
-    return c.bad(PLR_ERR_INVALID, "k must be at most 2^24 and a code pitch 2^23 bytes");
+  const int64_t most = (int64_t)1 << 23;
+  if (k > 2 * most || lda > most || ldb > most || ldsa > most || ldsb > most)
+    return c.bad(PLR_ERR_INVALID, "k must be at most 2^24 and a pitch of codes or scales 2^23 bytes");
   if (lda % 64 != 0 || ldb % 64 != 0 || lda < plr_mxfp_code_pitch(k) || ldb < plr_mxfp_code_pitch(k))
     return c.bad(PLR_ERR_INVALID, "code pitches must be multiples of 64 and at least plr_mxfp_code_pitch(k)");
   if (ldsa % 4 != 0 || ldsb % 4 != 0 || ldsa < plr_mxfp_scale_pitch(k) || ldsb < plr_mxfp_scale_pitch(k))
