@@ -56,8 +56,12 @@ __device__ __forceinline__ MaskRow mask_row(const Mask& m, int64_t row) {
   return {(unsigned)q, (unsigned)(p >> 32) ^ (m.key1 + kPhiloxW1), (unsigned)p};
 }
 
-// The 8 values of a group in a row: bit 4 i is 1 where value i is dropped.
-__device__ __forceinline__ unsigned drop_marks(const Mask& m, const MaskGroup& g, const MaskRow& r) {
+// The 8 values of a group in a row: halves w of the result hold 1 where values 2 w and 2 w + 1 are
+// dropped.
+struct DropWords {
+  unsigned w[4];
+};
+__device__ __forceinline__ DropWords drop_words(const Mask& m, const MaskGroup& g, const MaskRow& r) {
   unsigned c0 = g.a ^ r.a, c1 = g.b, c2 = r.b ^ g.c, c3 = r.c;
 #pragma unroll
   for (int i = 2; i < 10; ++i) {
@@ -77,14 +81,24 @@ __device__ __forceinline__ unsigned drop_marks(const Mask& m, const MaskGroup& g
     asm("v_pk_min_u16 %0, %1, %2" : "=v"(d) : "s"(one), "v"(d));
     return d;
   };
+  return {{drops(c0), drops(c1), drops(c2), drops(c3)}};
+}
+// The same as one word: bit 4 i is 1 where value i is dropped.
+__device__ __forceinline__ unsigned drop_marks(const Mask& m, const MaskGroup& g, const MaskRow& r) {
+  const DropWords d = drop_words(m, g, r);
   // bytes 0 and 2 of each word hold a mark: the even values' go to the bytes of one word, the
   // odd ones' to another's
-  const unsigned d0 = drops(c0), d1 = drops(c1), d2 = drops(c2), d3 = drops(c3);
-  const unsigned lo = __builtin_amdgcn_perm(d1, d0, 0x06020400u);  // d0.0 d1.0 d0.2 d1.2
-  const unsigned hi = __builtin_amdgcn_perm(d3, d2, 0x06020400u);
+  const unsigned lo = __builtin_amdgcn_perm(d.w[1], d.w[0], 0x06020400u);  // 0.0 1.0 0.2 1.2
+  const unsigned hi = __builtin_amdgcn_perm(d.w[3], d.w[2], 0x06020400u);
   const unsigned even = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   const unsigned odd = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
   return even | odd << 4;
+}
+// Two 16-bit values, the marked ones zeroed.
+__device__ __forceinline__ unsigned zero_dropped(unsigned pair, unsigned marks) {
+  unsigned m;
+  asm("v_pk_sub_u16 %0, 0, %1" : "=v"(m) : "v"(marks));
+  return pair & ~m;
 }
 // Nibble i is 0xF where value i is kept, 0 where it is dropped.
 __device__ __forceinline__ unsigned kept_nibbles(unsigned marks) { return ~((marks << 4) - marks); }

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "plr_internal.hpp"
 #include "plr_matmul.hpp"
@@ -48,18 +49,32 @@ struct Elem<_Float16> {
   static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
 };
 
-// V consecutive values, moved as 16-byte words where the caller knows them aligned.
+// V consecutive values, moved in words of 16 bytes whatever the row's alignment: the device's
+// global loads and stores need none (rows of 4100 bfloat16 start on 8-byte boundaries).
 template <typename T, int V>
-struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+struct Pack {
   T v[V];
 };
+typedef int v4w __attribute__((ext_vector_type(4), aligned(2)));
+template <int N>
+struct Words {
+  v4w w[N];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_whole(const T* p) {
+  constexpr int N = (int)sizeof(T) * V / 16;
+  Words<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.w[i] = reinterpret_cast<const v4w*>(p)[i];
+  return __builtin_bit_cast(Pack<T, V>, r);
+}
 
 // Columns c .. c + V of a row at p (p = the row's first value); those at `cols` and behind are 0.
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p, int64_t c, int64_t cols, bool whole) {
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p, int64_t c, int64_t cols) {
   Pack<T, V> r;
-  if (whole && c + V <= cols) {
-    r = *reinterpret_cast<const Pack<T, V>*>(p + c);
+  if (c + V <= cols) {
+    r = load_whole<T, V>(p + c);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = c + i < cols ? p[c + i] : T(0);
@@ -67,10 +82,12 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p, int64_t c, int64_t c
   return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_pack(T* p, int64_t c, int64_t cols, bool whole,
-                                           const Pack<T, V>& r) {
-  if (whole && c + V <= cols) {
-    *reinterpret_cast<Pack<T, V>*>(p + c) = r;
+__device__ __forceinline__ void store_pack(T* p, int64_t c, int64_t cols, const Pack<T, V>& r) {
+  if (c + V <= cols) {
+    constexpr int N = (int)sizeof(T) * V / 16;
+    const Words<N> w = __builtin_bit_cast(Words<N>, r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<v4w*>(p + c)[i] = w.w[i];
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -126,6 +143,40 @@ __device__ __forceinline__ unsigned encode8(const double (&v)[8], unsigned s) {
   return encode8(f, 127u);
 }
 
+// Pairs of 16-bit values are worked on as they lie, two to a word.
+template <typename T>
+constexpr bool kPairs = sizeof(T) == 2;
+template <typename T, int SEL>
+__device__ __forceinline__ unsigned encode_pair(unsigned old, unsigned pair, float sc) {
+  if constexpr (std::is_same<T, __bf16>::value) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(v2, pair), sc, SEL);
+  } else {
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(v2, pair), sc, SEL);
+  }
+}
+template <typename T>
+__device__ __forceinline__ unsigned encode_pairs(const unsigned (&w)[4], float sc) {
+  unsigned r = 0;
+  r = encode_pair<T, 0>(r, w[0], sc);
+  r = encode_pair<T, 1>(r, w[1], sc);
+  r = encode_pair<T, 2>(r, w[2], sc);
+  return encode_pair<T, 3>(r, w[3], sc);
+}
+// Larger magnitude of each half; the maximum so far is without signs.
+__device__ __forceinline__ unsigned pair_max(unsigned top, unsigned pair) {
+  unsigned r;
+  asm("v_pk_max_u16 %0, %1, %2" : "=v"(r) : "v"(top), "v"(pair & 0x7fff7fffu));
+  return r;
+}
+// mag_bits of the float that a 16-bit magnitude stands for.
+template <typename T>
+__device__ __forceinline__ unsigned half_mag_bits(unsigned half) {
+  if constexpr (std::is_same<T, __bf16>::value) return half << 16;
+  return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)half));
+}
+
 struct QuantArgs {
   const void* x;
   int64_t n, d, ldx;
@@ -134,7 +185,6 @@ struct QuantArgs {
   uint8_t* scales;
   int64_t lds;
   int64_t chunks;  // 128-column chunks of an output row that are written
-  int wide_load;   // rows of x start on 16-byte boundaries
   int tc_log2;     // a workgroup's tile is 2^tc_log2 chunks wide
   unsigned nbx;    // tiles across
   Mask mask;
@@ -168,14 +218,28 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
 #pragma unroll
   for (int u = 0; u < kQuantRows; ++u) {
     const int64_t r = row + (int64_t)u * rows;
-    if (r < a.n) in[u] = load_pack<T, 8>(x + r * a.ldx, c, a.d, a.wide_load);
+    if (r < a.n) in[u] = load_pack<T, 8>(x + r * a.ldx, c, a.d);
   }
 #pragma unroll
   for (int u = 0; u < kQuantRows; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;  // (a quad shares its row: its lanes leave together)
+    unsigned top = 0, s, w;
+    if constexpr (kPairs<T>) {
+      v4w raw = __builtin_bit_cast(v4w, in[u]);
+      unsigned pairs[4] = {(unsigned)raw.x, (unsigned)raw.y, (unsigned)raw.z, (unsigned)raw.w};
+      if (DROP) {
+        const DropWords d = drop_words(a.mask, group, mask_row(a.mask, r));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pairs[i] = zero_dropped(pairs[i], d.w[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = pair_max(top, pairs[i]);
+      top = (top & 0xffffu) > top >> 16 ? top & 0xffffu : top >> 16;
+      s = scale_byte(half_mag_bits<T>(quad_max(top)), 0.f);
+      w = s == 255u ? 0u : encode_pairs<T>(pairs, scale_value(s));
+    } else {
     W v[8];
-    unsigned top = 0;
     const unsigned drop = DROP ? drop_marks(a.mask, group, mask_row(a.mask, r)) : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -184,9 +248,9 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
       const unsigned b = mag_bits(v[i]);
       top = b > top ? b : top;
     }
-    top = quad_max(top);
-    const unsigned s = scale_byte(top, W(0));
-    const unsigned w = s == 255u ? 0u : encode8(v, s);
+    s = scale_byte(quad_max(top), W(0));
+    w = s == 255u ? 0u : encode8(v, s);
+    }
     if (c / 2 < a.ldc && chunk < a.chunks)
       *reinterpret_cast<unsigned*>(a.codes + r * a.ldc + c / 2) = w;
     if ((l16 & 3) == 0 && c / 32 < a.lds && chunk < a.chunks)
@@ -194,30 +258,117 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
   }
 }
 
+// 32 values of one column, V columns of them in `in`, to a block of the result's row `j`.
+template <typename T, int V>
+__device__ __forceinline__ void put_column_block(const QuantArgs& a, const Pack<T, V> (&in)[32], int k, int64_t j,
+                                                 int64_t blk) {
+  typedef typename Elem<T>::wide W;
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const unsigned b = mag_bits(Elem<T>::up(in[i].v[k]));
+    top = b > top ? b : top;
+  }
+  const unsigned s = scale_byte(top, W(0));
+  uint4 w;
+  unsigned* ww = reinterpret_cast<unsigned*>(&w);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    W v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::up(in[8 * q + i].v[k]);
+    ww[q] = s == 255u ? 0u : encode8(v, s);
+  }
+  *reinterpret_cast<uint4*>(a.codes + j * a.ldc + blk * 16) = w;
+  if (blk < a.lds) a.scales[j * a.lds + blk] = (uint8_t)s;
+}
+
 // Blocks along a column: row j of the result is column j of x.  A thread holds V = 16 bytes of
 // columns times 32 rows in registers -- so a block never leaves its thread --, 8 lanes cover 128
 // bytes of a row of x and the 8 groups of lanes 256 rows, so that a result row is written in
-// pieces of 128 bytes.
+// pieces of 128 bytes.  The columns behind the last whole V are left to workgroups of their own
+// (the last of a tile row), where a thread takes one column.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(64) void quantize_columns(QuantArgs a) {
-  typedef typename Elem<T>::wide W;
+__global__ __launch_bounds__(64, 2) void quantize_columns(QuantArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
   const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
   const int lane = threadIdx.x;
-  const int64_t c0 = ((int64_t)bx * 8 + (lane & 7)) * V;  // first column of x
-  const int64_t blk = (int64_t)by * 8 + (lane >> 3);      // block of 32 rows
+  const int64_t blk = (int64_t)by * 8 + (lane >> 3);  // block of 32 rows
   const int64_t r0 = blk * 32;
-  if (c0 >= a.d || blk * 16 >= a.ldc || blk >= a.chunks * 4) return;
+  const int64_t whole = a.d / V * V;
+  if (blk * 16 >= a.ldc || blk >= a.chunks * 4) return;
   const T* x = static_cast<const T*>(a.x);
+  if ((int64_t)bx * 8 * V >= whole) {
+    const int64_t c = whole + (lane & 7);
+    if (c >= a.d) return;
+    const MaskGroup group = DROP ? mask_group(a.mask, (unsigned)(c >> 3)) : MaskGroup{};
+    Pack<T, 1> in[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      in[i].v[0] = r0 + i < a.n ? x[(r0 + i) * a.ldx + c] : T(0);
+      if (DROP && (drop_marks(a.mask, group, mask_row(a.mask, r0 + i)) >> 4 * (c & 7) & 1)) in[i].v[0] = T(0);
+    }
+    put_column_block<T, 1>(a, in, 0, c, blk);
+    return;
+  }
+  const int64_t c0 = ((int64_t)bx * 8 + (lane & 7)) * V;  // first column of x
+  if (c0 >= whole) return;
+  const Pack<T, V> zero = {};
   Pack<T, V> in[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
-    if (r0 + i < a.n) {
-      in[i] = load_pack<T, V>(x + (r0 + i) * a.ldx, c0, a.d, a.wide_load);
-    } else {
+    // rows behind the last one repeat it here and are zeroed below
+    const int64_t r = r0 + i < a.n ? r0 + i : a.n - 1;
+    in[i] = load_whole<T, V>(x + r * a.ldx + c0);
+  }
+  if (r0 + 32 > a.n) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) in[i].v[k] = T(0);
+    for (int i = 0; i < 32; ++i)
+      if (r0 + i >= a.n) in[i] = zero;
+  }
+  if constexpr (kPairs<T>) {
+    // two columns at a time: both maxima in one word, then pairs of rows of either column
+    v4w raw[32];
+    const MaskGroup group = DROP ? mask_group(a.mask, (unsigned)(c0 >> 3)) : MaskGroup{};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      raw[i] = __builtin_bit_cast(v4w, in[i]);
+      if (DROP) {
+        const DropWords d = drop_words(a.mask, group, mask_row(a.mask, r0 + i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[i][k] = (int)zero_dropped((unsigned)raw[i][k], d.w[k]);
+        // row after row: 32 generator calls at once take more registers than there are
+        asm volatile("" : "+v"(raw[i]));
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = pair_max(top, (unsigned)raw[i][k]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned s = scale_byte(half_mag_bits<T>(h ? top >> 16 : top & 0xffffu), 0.f);
+        const float sc = scale_value(s);
+        uint4 w = uint4{0, 0, 0, 0};
+        if (s != 255u) {
+          unsigned* ww = reinterpret_cast<unsigned*>(&w);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            unsigned pairs[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              pairs[i] = __builtin_amdgcn_perm((unsigned)raw[8 * q + 2 * i + 1][k], (unsigned)raw[8 * q + 2 * i][k],
+                                               h ? 0x07060302u : 0x05040100u);
+            ww[q] = encode_pairs<T>(pairs, sc);
+          }
+        }
+        const int64_t j = c0 + 2 * k + h;
+        *reinterpret_cast<uint4*>(a.codes + j * a.ldc + blk * 16) = w;
+        if (blk < a.lds) a.scales[j * a.lds + blk] = (uint8_t)s;
+      }
+    }
+    return;
   }
   if (DROP) {
     const MaskGroup group = mask_group(a.mask, (unsigned)(c0 >> 3));
@@ -225,32 +376,14 @@ __global__ __launch_bounds__(64) void quantize_columns(QuantArgs a) {
     for (int i = 0; i < 32; ++i) {
       const unsigned drop = drop_marks(a.mask, group, mask_row(a.mask, r0 + i)) >> 4 * (c0 & 7);
 #pragma unroll
-      for (int k = 0; k < V; ++k)
+      for (int k = 0; k < V; ++k) {
         if (drop >> 4 * k & 1) in[i].v[k] = T(0);
+        asm volatile("" : "+v"(in[i].v[k]));
+      }
     }
   }
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    if (c0 + k >= a.d) break;
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const unsigned b = mag_bits(Elem<T>::up(in[i].v[k]));
-      top = b > top ? b : top;
-    }
-    const unsigned s = scale_byte(top, W(0));
-    uint4 w;
-    unsigned* ww = reinterpret_cast<unsigned*>(&w);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      W v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = Elem<T>::up(in[8 * q + i].v[k]);
-      ww[q] = s == 255u ? 0u : encode8(v, s);
-    }
-    *reinterpret_cast<uint4*>(a.codes + (c0 + k) * a.ldc + blk * 16) = w;
-    if (blk < a.lds) a.scales[(c0 + k) * a.lds + blk] = (uint8_t)s;
-  }
+  for (int k = 0; k < V; ++k) put_column_block<T, V>(a, in, k, c0 + k, blk);
 }
 
 struct DequantArgs {
@@ -260,7 +393,6 @@ struct DequantArgs {
   int64_t lds;
   void* out;
   int64_t n, d, ldo;
-  int wide_store;
   int tc_log2;
   unsigned nbx;
 };
@@ -295,7 +427,7 @@ __global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) 
     Pack<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = Elem<T>::down((W)q[i >> 1][i & 1] * sc);
-    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
+    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, o);
   }
 }
 
@@ -304,7 +436,6 @@ struct DropArgs {
   const void* x;
   void* out;
   int64_t n, d, ldx, ldo;
-  int wide_load, wide_store;
   int tc_log2;
   unsigned nbx;
   double scale;
@@ -326,7 +457,7 @@ __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
 #pragma unroll
   for (int u = 0; u < kQuantRows; ++u) {
     const int64_t r = row + (int64_t)u * rows;
-    if (r < a.n) in[u] = load_pack<T, 8>(static_cast<const T*>(a.x) + r * a.ldx, c, a.d, a.wide_load);
+    if (r < a.n) in[u] = load_pack<T, 8>(static_cast<const T*>(a.x) + r * a.ldx, c, a.d);
   }
   const W sc = (W)a.scale;
   const MaskGroup group = mask_group(a.mask, (unsigned)(c >> 3));
@@ -339,7 +470,7 @@ __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       o.v[i] = (drop >> 4 * i & 1) ? T(0) : Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc);
-    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, a.wide_store, o);
+    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, o);
   }
 }
 
@@ -514,12 +645,12 @@ int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned 
   a.lds = lds;
   // whole 128-column chunks are written as far as the pitches reach
   a.chunks = ceil_div(cols, 128);
-  a.wide_load = aligned(dx, 16) && ldx * (int64_t)size % 16 == 0;
   a.mask = mask;
   a.tc_log2 = 0;
   unsigned grid = 0;
   if (tr) {
-    const int64_t x = ceil_div(d, 8 * (16 / (int64_t)size)), y = ceil_div(a.chunks * 4, 8);
+    const int64_t v = 16 / (int64_t)size;  // columns a thread takes; what is over has its own workgroups
+    const int64_t x = ceil_div(d / v, 8) + (d % v != 0), y = ceil_div(a.chunks * 4, 8);
     if (!fits_launch(x, y, 64)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
     a.nbx = (unsigned)x;
     grid = (unsigned)(x * y);
@@ -568,7 +699,6 @@ int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, 
   a.n = n;
   a.d = d;
   a.ldo = ldo;
-  a.wide_store = aligned(dout, 16) && ldo * (int64_t)size % 16 == 0;
   const int64_t chunks = ceil_div(d, 128);
   a.tc_log2 = tile_log2(chunks);
   unsigned grid = 0;
@@ -609,8 +739,6 @@ int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned 
   a.d = d;
   a.ldx = ldx;
   a.ldo = ldo;
-  a.wide_load = aligned(dx, 16) && ldx * (int64_t)size % 16 == 0;
-  a.wide_store = aligned(dout, 16) && ldo * (int64_t)size % 16 == 0;
   const int64_t chunks = ceil_div(d, 128);
   a.tc_log2 = tile_log2(chunks);
   unsigned grid = 0;
