@@ -618,11 +618,16 @@ int packed_slots(const PackedFns* f, int blocks) {
 }
 
 // LDS: theta, partial dot products, residuals and (with dropout) marks of a tile, and in the end
-// 8 doubles a thread.
-size_t packed_lds(const PackedFns* f, int blocks, bool drop) {
-  const size_t rows = (size_t)packed_slots(f, blocks) * f->sets;
-  return std::max((size_t)f->threads * 8, (size_t)32 * f->stride + rows * ((blocks | 1) + 1)) *
-             sizeof(double) + (drop ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
+// 9 doubles a thread; of a row's widest and narrowest piece.
+size_t packed_lds(const PackedFns* f, int64_t row_blocks, bool drop) {
+  auto one = [&](int64_t blocks) {
+    const size_t rows = (size_t)packed_slots(f, (int)blocks) * f->sets;
+    return std::max((size_t)f->threads * 9, (size_t)32 * f->stride + rows * ((blocks | 1) + 1)) * sizeof(double) +
+           (drop ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
+  };
+  if (row_blocks <= kPackedFused) return one(row_blocks);
+  const int64_t over = row_blocks % kPackedPiece;
+  return std::max(one(kPackedPiece), over ? one(over) : 0);
 }
 
 const PackedFns* packed_fns_for(int64_t blocks) {
@@ -663,11 +668,15 @@ int plan_packed(plr_ctx* c, int64_t n) {
       PLR_HIP(c, hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
       int o = 0;
       PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(&o, f, pf->threads,
-                                                              packed_lds(pf, blocks, k == 1)));
+                                                              packed_lds(pf, c->row_blocks, k == 1)));
       occ = std::min(occ, o);
     }
     if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
-    c->packed_grid[k] = (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)c->num_cu * occ));
+    // pieces side by side share the device: fewer, longer workgroups leave fewer partials to add up
+    // (12000 x 16385: 97 -> 88 us a pass)
+    const int64_t wide = c->packed_sweeps ? c->row_blocks / kPackedPiece : 1;
+    c->packed_grid[k] =
+        (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)c->num_cu * occ / wide));
   }
   c->grid = std::max(c->packed_grid[0], c->packed_grid[1]);
   c->grid_nograd = c->packed_grid[2];
@@ -757,7 +766,8 @@ int alloc_workspace(plr_ctx* c) {
     PLR_HIP(c, hipMalloc(&c->d_zparts, (size_t)c->zstride * c->nteams * c->team_blocks *
                                            plr::kTeamWaves * sizeof(double)));
   } else if ((c->blocked || c->packed_sweeps) && n > 0) {
-    PLR_HIP(c, hipMalloc(&c->d_z, (size_t)n * sizeof(double)));
+    const int64_t parts = c->packed_sweeps ? ceil_div(c->row_blocks, kPackedPiece) : 1;
+    PLR_HIP(c, hipMalloc(&c->d_z, (size_t)n * parts * sizeof(double)));
     PLR_HIP(c, hipMalloc(&c->d_res, (size_t)n * sizeof(double)));
   }
   PLR_HIP(c, hipHostMalloc(&c->h_theta, (size_t)(c->theta_len + 8) * sizeof(double),
@@ -835,7 +845,6 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
   a.pitch = c->pitch;
   a.loss_mode = pa.loss_mode;
   a.identity_link = pa.identity_link;
-  a.z_accumulate = 0;
   a.kept = 1.;
   a.mask = plr_mx::Mask{0, 0, 0, 0, 0};
   const bool drop = grad && c->drop_on;
@@ -848,36 +857,25 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
   const PackedFns* pf = c->packed_fns;
   const int grid = c->packed_grid[!grad ? 2 : drop ? 1 : 0];
   *parts = *loss_parts = grid;
-  auto launch = [&](packed_fn f, int blk0, int blocks) {
-    a.blk0 = blk0;
-    a.blocks = blocks;
-    a.slots = packed_slots(pf, blocks);
-    a.groups = ceil_div(c->n, (int64_t)a.slots * plr::kPackedR);
-    // a lane sums up to 32 of a row's partials: the fewer waves evaluate row terms the better
-    a.lanes_per_row = 1;
-    while (a.lanes_per_row < plr::kWave && a.lanes_per_row * 32 < blocks) a.lanes_per_row *= 2;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(pf->threads), packed_lds(pf, blocks, drop), c->stream, a);
+  a.piece = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
+  a.most_slots = packed_slots(pf, 1);
+  const int pieces = (int)ceil_div(c->row_blocks, a.piece);
+  const size_t lds = packed_lds(pf, c->row_blocks, drop);
+  auto launch = [&](packed_fn f) {
+    hipLaunchKernelGGL(f, dim3(grid, pieces), dim3(pf->threads), lds, c->stream, a);
     return hipGetLastError();
   };
   if (!c->packed_sweeps) {
-    PLR_HIP(c, launch(grad ? c->packed_fns->grad[drop] : c->packed_fns->eval, 0, (int)c->row_blocks));
+    PLR_HIP(c, launch(grad ? pf->grad[drop] : pf->eval));
     return PLR_OK;
   }
-  for (int64_t b = 0; b < c->row_blocks; b += kPackedPiece) {
-    const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
-    a.z_accumulate = b > 0;
-    PLR_HIP(c, launch(kPackedDot[drop], (int)b, w));
-  }
-  hipLaunchKernelGGL(plr::residual_pass, dim3(c->res_grid), dim3(256), 0, c->stream,
-                     (const double*)c->d_z, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
-                     c->d_part_loss, c->n, pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res,
-                     0, 0, (int64_t)0);
+  PLR_HIP(c, launch(kPackedDot[drop]));
+  hipLaunchKernelGGL(plr::packed_residual, dim3(c->res_grid), dim3(256), 0, c->stream, (const double*)c->d_z,
+                     pieces, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out, c->d_part_loss, c->n,
+                     pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res);
   PLR_HIP(c, hipGetLastError());
   *loss_parts = c->res_grid;
-  for (int64_t b = 0; grad && b < c->row_blocks; b += kPackedPiece) {
-    const int w = (int)std::min<int64_t>(kPackedPiece, c->row_blocks - b);
-    PLR_HIP(c, launch(kPackedAxpy[drop], (int)b, w));
-  }
+  if (grad) PLR_HIP(c, launch(kPackedAxpy[drop]));
   return PLR_OK;
 }
 

@@ -37,16 +37,13 @@ struct PackedArgs {
   double* part_loss;      // [grid]
   double* part_res;       // [grid] or nullptr
   double* h_out;          // n or nullptr
-  double* z_buf;          // kPassDot: n
+  double* z_buf;          // kPassDot: [pieces][n], each piece's part of the dot products
   const double* res_in;   // kPassAxpy: n
   int64_t n;
-  int64_t groups;         // of R row sets: ceil(n / (slots * R))
   int64_t row_blocks;     // blocks of a stored row
   int64_t pitch;          // doubles per row of part_g
-  int blk0, blocks;       // the blocks this launch covers
-  int slots;              // rows side by side: threads / blocks
-  int lanes_per_row;      // threads that sum a row's partials (a power of two, at most 64)
-  int z_accumulate;
+  int piece;              // most blocks a workgroup takes; blockIdx.y is its piece of the row
+  int most_slots;         // most rows side by side
   unsigned loss_mode;
   int identity_link;
   double kept;            // dropout: the factor of what is kept
@@ -109,37 +106,38 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
   static_assert(SR % R == 0, "whole groups of row sets");
   extern __shared__ double sm[];
   const int tid = threadIdx.x;
-  const int max_rows = a.slots * SR;  // rows of a tile
-  const int zpitch = a.blocks | 1; // odd: a row's partials start on another bank than the next one's
+  const int blk0 = (int)blockIdx.y * a.piece;
+  const int blocks = min(a.piece, (int)a.row_blocks - blk0);
+  const int slots = min(NT / blocks, a.most_slots);
+  const int max_rows = slots * SR;   // rows of a tile
+  const int zpitch = blocks | 1;     // odd: a row's partials start on another bank than the next one's
   v2d* const thl = reinterpret_cast<v2d*>(sm);  // [16][STRIDE]: columns 2i, 2i + 1
   double* const zl = sm + 32 * STRIDE;          // [max_rows][zpitch]
   double* const rl = zl + (size_t)max_rows * zpitch;  // [max_rows]
   unsigned* const ml = reinterpret_cast<unsigned*>(rl + max_rows);  // [SR][NT]: dropped values
-  const int slot = tid / a.blocks, blk = tid - slot * a.blocks;
-  const bool active = slot < a.slots;
+  const int slot = tid / blocks, blk = tid - slot * blocks;
+  const bool active = slot < slots;
   const int lane = tid & (kWave - 1), wave = tid / kWave;
+  // a lane sums up to 32 of a row's partials: the fewer waves evaluate row terms the better
+  int per = 1;
+  while (per < kWave && per * 32 < blocks) per *= 2;
   double acc[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) acc[i] = 0.;
-  if (MODE != kPassAxpy) {
-    const v2d* src = reinterpret_cast<const v2d*>(a.theta + (int64_t)a.blk0 * 32);
-    for (int e = tid; e < 16 * a.blocks; e += NT) thl[(e & 15) * STRIDE + (e >> 4)] = src[e];
-    __syncthreads();
-  }
   plr_mx::MaskGroup group[4];
   if (DROP) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) group[q] = plr_mx::mask_group(a.mask, (unsigned)((a.blk0 + blk) * 4 + q));
+    for (int q = 0; q < 4; ++q) group[q] = plr_mx::mask_group(a.mask, (unsigned)((blk0 + blk) * 4 + q));
   }
   RowSums sums;
   const double bias = a.theta_bias ? *a.theta_bias : 0.;
 
   // R row sets from set `set` on (behind the last row lie readable zeros: they count nothing).
-  const unsigned at_lane = (unsigned)((active ? slot : 0) * a.row_blocks + a.blk0 + blk);
+  const unsigned at_lane = (unsigned)((active ? slot : 0) * a.row_blocks + blk0 + blk);
   auto load = [&](int64_t set, PackedLoads<R>& t) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int64_t at = (set + r) * a.slots * a.row_blocks;  // the same for all threads
+      const int64_t at = (set + r) * slots * a.row_blocks;  // the same for all threads
       t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
       t.scales[r] = (a.scales + at)[at_lane];
     }
@@ -148,7 +146,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
   auto drop = [&](int64_t set, PackedTile<R>& t, unsigned (&marks)[R]) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const plr_mx::MaskRow mr = plr_mx::mask_row(a.mask, (set + r) * a.slots + slot);
+      const plr_mx::MaskRow mr = plr_mx::mask_row(a.mask, (set + r) * slots + slot);
       const unsigned m0 = plr_mx::drop_marks(a.mask, group[0], mr);
       const unsigned m1 = plr_mx::drop_marks(a.mask, group[1], mr);
       const unsigned m2 = plr_mx::drop_marks(a.mask, group[2], mr);
@@ -182,11 +180,17 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
 
   // The workgroup's share: consecutive groups of R row sets, shares differing by one at most, in
   // tiles of up to SR sets.
-  const int64_t share = a.groups / gridDim.x, longer = a.groups - share * gridDim.x;
+  const int64_t groups = (a.n + (int64_t)slots * R - 1) / ((int64_t)slots * R);
+  const int64_t share = groups / gridDim.x, longer = groups - share * gridDim.x;
   const int64_t first = blockIdx.x * share + min((int64_t)blockIdx.x, longer);
   const int64_t end = (first + share + ((int64_t)blockIdx.x < longer ? 1 : 0)) * R;
   PackedLoads<R> nxt;
   if (first * R < end) load(first * R, nxt);
+  if (MODE != kPassAxpy) {
+    const v2d* src = reinterpret_cast<const v2d*>(a.theta + (int64_t)blk0 * 32);
+    for (int e = tid; e < 16 * blocks; e += NT) thl[(e & 15) * STRIDE + (e >> 4)] = src[e];
+    __syncthreads();
+  }
   for (int64_t set0 = first * R; set0 < end; set0 += SR) {
     const int sets = (int)min((int64_t)SR, end - set0);
     const bool more = set0 + SR < end;
@@ -223,28 +227,28 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
         if (active) {
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            zl[((s + r) * a.slots + slot) * zpitch + blk] = (part[r][0] + part[r][1]) * tile_scale(cur, r);
+            zl[((s + r) * slots + slot) * zpitch + blk] = (part[r][0] + part[r][1]) * tile_scale(cur, r);
         }
       }
       __syncthreads();
-      const int rows = sets * a.slots;
-      const int per = a.lanes_per_row, sub = tid & (per - 1);
+      const int rows = sets * slots;
+      const int sub = tid & (per - 1);
       for (int q0 = 0; q0 < rows; q0 += NT / per) {
         const int q = q0 + tid / per;
         double z = 0.;
         if (q < rows) {
           const double* p = zl + q * zpitch;
 #pragma unroll 4
-          for (int b = sub; b < a.blocks; b += per) z += p[b];
+          for (int b = sub; b < blocks; b += per) z += p[b];
         }
         for (int m = 1; m < per; m <<= 1) z += __shfl_xor(z, m, kWave);
-        const int64_t row = set0 * a.slots + q;
+        const int64_t row = set0 * slots + q;
         if (q < rows && sub == 0) {
           double res = 0.;
           if (row < a.n) {
             if (DROP) z *= a.kept;
             if (MODE == kPassDot) {
-              a.z_buf[row] = a.z_accumulate ? a.z_buf[row] + z : z;
+              a.z_buf[(int64_t)blockIdx.y * a.n + row] = z;
             } else {
               double h, l;
               const double yv = a.y ? a.y[row] : 0.;
@@ -274,14 +278,14 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
           }
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            const int64_t row = (set0 + s + r) * a.slots + slot;
+            const int64_t row = (set0 + s + r) * slots + slot;
             w[r] = active && row < a.n ? a.res_in[row] * tile_scale(cur, r) : 0.;
           }
         } else {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             if (DROP) drop_again(cur, r, ml[(s + r) * NT + tid]);
-            w[r] = active ? rl[(s + r) * a.slots + slot] * tile_scale(cur, r) : 0.;
+            w[r] = active ? rl[(s + r) * slots + slot] * tile_scale(cur, r) : 0.;
           }
         }
 #pragma unroll
@@ -292,25 +296,54 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
     }
   }
   if (GRAD) {
-    // the slots' sums, eight columns at a time, in slot order
+    // The slots' sums, eight columns at a time: `share8` threads to a column, each in slot order,
+    // then among themselves.  (9 doubles per thread keep a column's slots on different banks.)
+    int share8 = 1;
+    while (share8 < kWave && share8 * 2 * blocks * 8 <= NT && share8 < slots) share8 *= 2;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       if (active) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sm[tid * 8 + i] = acc[8 * q + i];
+        for (int i = 0; i < 8; ++i) sm[tid * 9 + i] = acc[8 * q + i];
       }
       __syncthreads();
-      for (int e = tid; e < a.blocks * 8; e += NT) {
-        const int b = e >> 3, i = e & 7;
+      for (int e0 = 0; e0 < blocks * 8; e0 += NT / share8) {
+        const int e = e0 + tid / share8, b = e >> 3, i = e & 7;
         double g = 0.;
-        for (int s = 0; s < a.slots; ++s) g += sm[(s * a.blocks + b) * 8 + i];
-        a.part_g[(int64_t)blockIdx.x * a.pitch + (int64_t)(a.blk0 + b) * 32 + 8 * q + i] = g;
+        if (b < blocks)
+          for (int s = tid & (share8 - 1); s < slots; s += share8) g += sm[(s * blocks + b) * 9 + i];
+        for (int m = 1; m < share8; m <<= 1) g += __shfl_xor(g, m, kWave);
+        if (b < blocks && (tid & (share8 - 1)) == 0)
+          a.part_g[(int64_t)blockIdx.x * a.pitch + (int64_t)(blk0 + b) * 32 + 8 * q + i] = g;
       }
       __syncthreads();
     }
   }
   if (MODE == kPassFused) emit_row_sums<NT / kWave>(sums, lane, wave, a.part_loss, a.part_res);
+}
+
+// Between the two sweeps over wide rows: a row's dot product from its pieces' parts, in their
+// order, and its terms.
+__global__ __launch_bounds__(256) void packed_residual(const double* __restrict__ z, int pieces,
+                                                       const double* __restrict__ y, double* __restrict__ res,
+                                                       double* __restrict__ h_out, double* __restrict__ part_loss,
+                                                       int64_t n, unsigned loss_mode, int identity_link,
+                                                       const double* __restrict__ theta_bias,
+                                                       double* __restrict__ part_res) {
+  const double bias = theta_bias ? *theta_bias : 0.;
+  RowSums sums;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    double s = 0., h, l;
+    for (int p = 0; p < pieces; ++p) s += z[(int64_t)p * n + i];
+    const double yv = y ? y[i] : 0.;
+    row_terms(s + bias, yv, loss_mode, identity_link, h, l);
+    if (res) res[i] = h - yv;
+    if (h_out) store_h(h_out + i, h);
+    sums.loss += l;
+    sums.res += h - yv;
+  }
+  emit_row_sums<4>(sums, threadIdx.x & (kWave - 1), threadIdx.x / kWave, part_loss, part_res);
 }
 
 }  // namespace plr
