@@ -141,6 +141,7 @@ void logistic_regression_gpu::dgd_learning() {
     // (one fused pass and the two all-reduces of lr.cpp:331-335 per round
     // instead of n_local passes)
     double loss_sum = 0.;
+    check(shard.round(gpu, (int)get_worker_id(), rd), "plr_set_dropout");
     {
       gpu_turn_guard mine(turn);  // several workers on the GPU: one pass at a time
       lap(t, phase[1]);
@@ -183,6 +184,7 @@ void logistic_regression_gpu::solve() {
     load_and_parse(input);
     upload();
   }
+  check(shard.resident(gpu), "plr_pack_data");
   std::cout << "shard on the device: " << plr_kernel_info(gpu) << std::endl;
   paracel_sync();
   if (learning_method == "dgd") {

@@ -15,6 +15,7 @@
 #include "../../include/plr.h"
 #include "gpu_turn.hpp"
 #include "paralg_lite.hpp"
+#include "shard_options.hpp"
 
 namespace plr_ps {
 
@@ -35,6 +36,8 @@ class logistic_regression_gpu : public paralg {
   // theta the first round starts from; by default the reference's
   // random_double_list (utils.hpp:116-131: libc random()/RAND_MAX in (0,1))
   void set_theta0(const std::vector<double>& t0) { theta0 = t0; }
+  // 4-bit storage of the training shard, dropout in its rounds
+  void set_shard_options(const shard_options& o) { shard = o; }
 
   virtual void solve();         // lr.cpp:301-319
   void dgd_learning();          // lr.cpp:109-152
@@ -70,6 +73,7 @@ class logistic_regression_gpu : public paralg {
   int64_t pred_dim = 0;
   plr_ctx* gpu = nullptr;
   gpu_turn turn;
+  shard_options shard;
   double round_sec = 0.;
 };
 

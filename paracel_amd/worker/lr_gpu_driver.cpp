@@ -2,7 +2,8 @@
 // alg/classification/logistic_regression/lr_driver.cpp:34-78: the same two
 // flags (--server_info, --cfg_file), the same JSON keys (training_input,
 // test_input, predict_input, output, update_file, update_func, method, rounds,
-// alpha, beta, debug) and the same call order solve -> calc_loss -> test ->
+// alpha, beta, debug; optional beyond them: storage, dropout, dropout_seed, shard_options.hpp) and
+// the same call order solve -> calc_loss -> test ->
 // predict -> dump_result.
 //
 // A second mode serves the end-to-end benchmark: --synthetic SEED,N,D,SCALE
@@ -38,6 +39,7 @@ int main(int argc, char** argv) {
                                                            update_func = "lr_theta_update";
   int rounds = 100, device = 0, worker_id = 0, worker_sz = 1;
   double alpha = 0.002, beta = 0.1;
+  std::map<std::string, std::string> shard_kv;  // --synthetic's storage, dropout, dropout_seed
   for (int i = 1; i < argc; ++i) {
     std::string a = argv[i], v;
     const size_t eq = a.find('=');
@@ -58,6 +60,7 @@ int main(int argc, char** argv) {
     else if (a == "--update_file") update_file = v;
     else if (a == "--update_func") update_func = v;
     else if (a == "--device") device = atoi(v.c_str());
+    else if (a == "--storage" || a == "--dropout" || a == "--dropout_seed") shard_kv[a.substr(2)] = v;
     else if (a == "--worker_id") worker_id = atoi(v.c_str());
     else if (a == "--worker_sz") worker_sz = atoi(v.c_str());
     else {
@@ -73,6 +76,7 @@ int main(int argc, char** argv) {
       double scale;
       if (sscanf(synthetic.c_str(), "%llx,%lld,%lld,%lf", &seed, &n, &d, &scale) != 4)
         throw std::invalid_argument("--synthetic wants SEEDHEX,N,D,SCALE");
+      const auto shard = plr_ps::shard_options::from(shard_kv);
       logistic_regression_gpu lr(server_info, "", "", update_file, update_func, "dgd", rounds,
                                  alpha, beta, false, device, worker_id, worker_sz);
       const long long lo = n * worker_id / worker_sz, hi = n * (worker_id + 1) / worker_sz;
@@ -86,6 +90,7 @@ int main(int argc, char** argv) {
         lr.set_samples(X.data(), m, d, d, y.data());
       }
       if (theta0 == "zero") lr.set_theta0(std::vector<double>(d, 0.));
+      lr.set_shard_options(shard);
       lr.solve();
       const double loss = lr.calc_loss();
       const double sec = lr.round_seconds(), kms = lr.gpu_kernel_ms();
@@ -101,6 +106,7 @@ int main(int argc, char** argv) {
       return 0;
     }
     auto kv = parse_flat_json(cfg_file);
+    const auto shard = plr_ps::shard_options::from(kv);
     logistic_regression_gpu lr(server_info, need(kv, "training_input"), need(kv, "output"),
                                need(kv, "update_file"), need(kv, "update_func"),
                                need(kv, "method"), atoi(need(kv, "rounds").c_str()),
@@ -108,6 +114,7 @@ int main(int argc, char** argv) {
                                need(kv, "debug") == "true", device, worker_id, worker_sz);
     if (theta0 == "zero")
       lr.set_theta0(std::vector<double>(plr_ps::csv_row_width(need(kv, "training_input")), 0.));
+    lr.set_shard_options(shard);
     lr.solve();
     std::cout.precision(17);
     std::cout << "final loss: " << lr.calc_loss() << std::endl;

@@ -78,6 +78,7 @@ void ridge_regression_gpu::batch_learning() {
   for (int rd = 0; rd < rounds; ++rd) {
     theta = paracel_read<std::vector<double> >("theta");
     paracel_sync_arrive();  // theta is read (see lr_gpu.cpp)
+    check(shard.round(gpu, (int)get_worker_id(), rd), "plr_set_dropout");
     {
       gpu_turn_guard mine(turn);  // several workers on the GPU: one pass at a time
       check(plr_dgd_delta_linear(gpu, theta.data(), alpha, beta, delta.data(), nullptr),
@@ -93,6 +94,7 @@ void ridge_regression_gpu::batch_learning() {
 
 void ridge_regression_gpu::solve() {
   load_and_upload(input);
+  check(shard.resident(gpu), "plr_pack_data");
   std::cout << "shard on the device: " << plr_kernel_info(gpu) << std::endl;
   paracel_sync();
   batch_learning();

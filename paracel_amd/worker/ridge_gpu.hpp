@@ -24,6 +24,7 @@
 #include "../../include/plr.h"
 #include "gpu_turn.hpp"
 #include "paralg_lite.hpp"
+#include "shard_options.hpp"
 
 namespace plr_ps {
 
@@ -36,6 +37,8 @@ class ridge_regression_gpu : public paralg {
   virtual ~ridge_regression_gpu();
 
   void set_theta0(const std::vector<double>& t0) { theta0 = t0; }
+  // 4-bit storage of the training shard, dropout in its rounds
+  void set_shard_options(const shard_options& o) { shard = o; }
 
   virtual void solve();         // ridge.hpp:55-61 with the batch trainer
   void batch_learning();        // full-batch rounds (see the note above)
@@ -62,6 +65,7 @@ class ridge_regression_gpu : public paralg {
   int64_t pred_dim = 0;
   plr_ctx* gpu = nullptr;
   gpu_turn turn;
+  shard_options shard;
 };
 
 }  // namespace plr_ps

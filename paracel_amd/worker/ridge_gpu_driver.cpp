@@ -43,6 +43,7 @@ int main(int argc, char** argv) {
   plr_ps::limit_hw_queues_of_gpu_sharers(worker_sz);  // before the first GPU call
   try {
     auto kv = plr_ps::parse_flat_json(cfg_file);
+    const auto shard = plr_ps::shard_options::from(kv);
     plr_ps::ridge_regression_gpu solver(
         server_info, need(kv, "training_input"), need(kv, "output"), need(kv, "update_file"),
         need(kv, "update_func"), atoi(need(kv, "rounds").c_str()),
@@ -51,6 +52,7 @@ int main(int argc, char** argv) {
     if (theta0 == "zero")
       solver.set_theta0(
           std::vector<double>(plr_ps::csv_row_width(need(kv, "training_input")), 0.));
+    solver.set_shard_options(shard);
     solver.solve();
     std::cout.precision(17);
     std::cout << "final loss: " << solver.calc_loss() << std::endl;
