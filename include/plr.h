@@ -266,9 +266,12 @@ int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, 
  * column k and the end of its chunk must be 0 and their scales not 255 (as
  * plr_mxfp_quantize leaves them).  da and db 16-byte, dsa and dsb 4-byte
  * aligned.
+ * m and n are at most 2^31, k 2^24, the four pitches 2^23 bytes, and C's tiles
+ * of 128 x 128 must fit one launch (8388607 of them).
  *   drop (nullable)  dropout of C: a gradient with respect to a dropped A.
- *   workspace  plr_mxfp_matmul_workspace(m, n, k) bytes of device memory,
- *        16-byte aligned, used while the call's kernels run (0: may be NULL). */
+ *   workspace  plr_mxfp_matmul_workspace(m, n, k) bytes of device memory.  0
+ *        for every size: each sum is finished where it is formed; the
+ *        arguments keep a caller's program as it is should one ask for some. */
 int64_t plr_mxfp_matmul_workspace(int64_t m, int64_t n, int64_t k);
 int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64_t k,
                     const uint8_t* da, int64_t lda, const uint8_t* dsa, int64_t ldsa,

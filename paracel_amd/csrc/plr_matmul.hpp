@@ -24,7 +24,7 @@ struct MatmulArgs {
   int64_t ldc;
   float alpha;
   float kept;  // dropout: the factor of what is kept
-  int wide_store;  // rows of c start on 16-byte boundaries
+  int64_t row0, col0;  // where c's first element stands in the matrix that the mask belongs to
   Mask mask;
 };
 
@@ -41,14 +41,25 @@ __device__ __forceinline__ v4f mfma(v4i a, v4i b, v4f c, int sa, int sb) {
 
 // ------------------------------------------------------------------- epilogue
 template <typename T>
-struct alignas(16) Out8 {
+struct Out8 {
   T v[8];
 };
+// 16 bytes at a time on any alignment (the device's global stores need none)
+typedef int v4w __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ void store_whole(T* c, const Out8<T>& o) {
+  struct Words {
+    v4w w[sizeof(T) / 2];
+  };
+  const Words w = __builtin_bit_cast(Words, o);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<v4w*>(c)[i] = w.w[i];
+}
 
 // Columns j .. j + 7 of row i (j a multiple of 8): factor, dropout, one rounding.
 template <typename T, bool DROP>
 __device__ __forceinline__ Out8<T> finish8(const MatmulArgs& p, int64_t i, int64_t j, v4f lo, v4f hi) {
-  const unsigned drops = DROP ? drop_marks(p.mask, i, (unsigned)(j >> 3)) : 0u;
+  const unsigned drops = DROP ? drop_marks(p.mask, i + p.row0, (unsigned)((j + p.col0) >> 3)) : 0u;
   Out8<T> o;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -61,8 +72,7 @@ __device__ __forceinline__ Out8<T> finish8(const MatmulArgs& p, int64_t i, int64
 
 // A wave's 16 x (16 FN) piece of C, rows i0 .., columns j0 ..; lane (r16, q) holds columns
 // 32 (y / 2) + 8 q .. + 7 of row r16 in acc[y], acc[y + 1] (y even).  Tiles that lie inside C are
-// stored as they are held; those at its edge, or on rows without alignment, go through 1 KB of LDS
-// per wave and 32 columns, so that the code with the comparisons is there once and not for every
+// stored as they are held; those at its edge go through 1 KB of LDS per wave and 32 columns, so that the code with the comparisons is there once and not for every
 // register.
 template <typename T, bool DROP, int FN>
 __device__ __forceinline__ void store_piece(const MatmulArgs& p, int64_t i0, int64_t j0, const v4f* acc, int r16,
@@ -70,8 +80,7 @@ __device__ __forceinline__ void store_piece(const MatmulArgs& p, int64_t i0, int
   T* c = static_cast<T*>(p.c) + (i0 + r16) * p.ldc + j0 + q * 8;
 #pragma unroll
   for (int y = 0; y < FN; y += 2)
-    *reinterpret_cast<Out8<T>*>(c + y * 16) =
-        finish8<T, DROP>(p, i0 + r16, j0 + y * 16 + q * 8, acc[y], acc[y + 1]);
+    store_whole(c + y * 16, finish8<T, DROP>(p, i0 + r16, j0 + y * 16 + q * 8, acc[y], acc[y + 1]));
 }
 template <typename T, bool DROP, int FN>
 __device__ __forceinline__ void store_edge_piece(const MatmulArgs& p, int64_t i0, int64_t j0, const v4f* acc,
@@ -145,7 +154,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
   constexpr int FM = WM / 16, FN = WN / 16;        // 16-row pieces of a wave
   constexpr int LA = BM * 4 / NT, LB = BN * 4 / NT;  // asynchronous loads per thread and step
   constexpr int ROWS = BM + BN;
-  static_assert(ROWS == NT, "four words of scales per row and group, one load per thread and step");
+  // a group's scales: a quarter of the rows per step, 16 rows of four words to a wave's load; waves
+  // that are over repeat the first ones'
+  constexpr int UNITS = ROWS / 64;
+  static_assert(UNITS <= NT / 64 && ROWS % 64 == 0, "one load of scales per thread and step");
   static_assert(LA + LB <= FM && FN <= FM && FM >= 4, "a step's loads and reads fit its rows of instructions");
   __shared__ v4i stage[4][ROWS * 4];
   __shared__ v4i scale[3][ROWS];
@@ -177,17 +189,18 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
     if (i < LA) copy_to_lds(abase + at, aoff[i], to);
     else copy_to_lds(bbase + at, boff[i - LA], to);
   };
-  // a group's scales: load i brings the words of steps k .. k + 3 (the last step's again behind
-  // the end) of rows ROWS / 4 * i + tid / 4 into ring place `to`
+  // load i brings the words of steps k .. k + 3 (the last step's again behind the end) of a quarter
+  // of the rows into ring place `to`
+  const int unit = wave < UNITS ? wave : wave - UNITS;
   const uint8_t* srow[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = ROWS / 4 * i + (tid >> 2);
+    const int r = ROWS / 4 * i + unit * 16 + (lane >> 2);
     srow[i] = r < BM ? p.sa + min(m0 + r, p.m - 1) * p.ldsa : p.sb + min(n0 + r - BM, p.n - 1) * p.ldsb;
   }
-  const unsigned lds1 = lds_address(&scale[0][0]) + (unsigned)wave * 256u;
+  const unsigned lds1 = lds_address(&scale[0][0]) + (unsigned)unit * 256u;
   auto fill_scales = [&](int to, int k, int i) {
-    copy_word_to_lds(srow[i] + (int64_t)min(k + (tid & 3), kc - 1) * 4,
+    copy_word_to_lds(srow[i] + (int64_t)min(k + (lane & 3), kc - 1) * 4,
                      lds1 + (unsigned)(to * ROWS * 16 + i * ROWS * 4));
   };
 
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
 #undef PLR_STEP
   // the loads of the steps behind the last one still write to LDS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if (p.wide_store && m0 + BM <= p.m && n0 + BN <= p.n) {
+  if (m0 + BM <= p.m && n0 + BN <= p.n) {
 #pragma unroll
     for (int x = 0; x < FM; ++x)
       store_piece<T, DROP, FN>(p, m0 + wm + 16 * x, n0 + wn, acc[x], r16, q);
@@ -297,16 +310,19 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
 }
 
 // ------------------------------------------------------------------- few rows on one side
-// At most 64 rows of the one operand ("few") against many of the other: bound by the bytes of the
-// many, which are read once, straight into the instruction's operands.  A workgroup owns 16 FX rows
-// of the many; its W waves divide k, and their sums meet in LDS in wave order.  Codes of four
-// chunks are requested at once: 256 consecutive bytes of a row.
+// A few rows of the one operand ("few") against many of the other: bound by the bytes of the many,
+// which are read once, straight into the instruction's operands.  A workgroup owns 16 FX rows of
+// the many and 16 FY of the few; its W waves divide k, and their sums meet in LDS in wave order.
+// Codes of four chunks are requested at once: 256 consecutive bytes of a row.  The same, in
+// pieces of 64 x 32 and 32 x 32, serves small products, which have too few large tiles to fill the
+// device.  Rows a power of two of bytes apart meet in the same channels of the L2 cache
+// (256 x 256 x 16384: 17 us, where its bytes alone are 4): 16 waves to a piece make it slower.
 struct FewArgs {
   MatmulArgs p;
   const uint8_t *x, *y, *sx, *sy;  // many, few
   int64_t ldx, ldy, ldsx, ldsy;
   int64_t rows;  // of x
-  int few;       // rows of y
+  int64_t few;   // rows of y
 };
 
 struct alignas(4) Words4 {
@@ -318,7 +334,7 @@ __global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
   __shared__ v4f part[W > 1 ? W - 1 : 1][FX * FY][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
-  const int64_t x0 = (int64_t)blockIdx.x * (16 * FX);
+  const int64_t x0 = (int64_t)blockIdx.x * (16 * FX), y0 = (int64_t)blockIdx.y * (16 * FY);
   const uint8_t *px[FX], *qx[FX], *py[FY], *qy[FY];
 #pragma unroll
   for (int f = 0; f < FX; ++f) {
@@ -328,9 +344,9 @@ __global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
   }
 #pragma unroll
   for (int f = 0; f < FY; ++f) {
-    const int r = min(16 * f + r16, a.few - 1);
-    py[f] = a.y + (int64_t)r * a.ldy + q * 16;
-    qy[f] = a.sy + (int64_t)r * a.ldsy;
+    const int64_t r = min(y0 + 16 * f + r16, a.few - 1);
+    py[f] = a.y + r * a.ldy + q * 16;
+    qy[f] = a.sy + r * a.ldsy;
   }
   v4f acc[FX][FY];
 #pragma unroll
@@ -398,20 +414,20 @@ __global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
 #pragma unroll
         for (int w = 0; w < W - 1; ++w) acc[x][y] += part[w][x * FY + y][lane];
   }
-  // lane (r16, q): rows x0 + 16 x + 4 q .. + 3 of the many, row 16 y + r16 of the few
+  // lane (r16, q): rows x0 + 16 x + 4 q .. + 3 of the many, row y0 + 16 y + r16 of the few
 #pragma unroll
   for (int x = 0; x < FX; ++x)
 #pragma unroll
     for (int y = 0; y < FY; ++y) {
-      const int64_t xr = x0 + 16 * x + 4 * q, yr = 16 * y + r16;
+      const int64_t xr = x0 + 16 * x + 4 * q, yr = y0 + 16 * y + r16;
       if (xr >= a.rows || yr >= a.few) continue;
       unsigned drops = 0;
-      if (DROP && !SWAP) drops = drop_marks(a.p.mask, yr, (unsigned)(xr >> 3)) >> 4 * (xr & 7);
+      if (DROP && !SWAP) drops = drop_marks(a.p.mask, yr + a.p.row0, (unsigned)((xr + a.p.col0) >> 3)) >> 4 * (xr & 7);
       T out[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v = a.p.alpha * acc[x][y][e];
-        if (DROP && SWAP) drops = drop_marks(a.p.mask, xr + e, (unsigned)(yr >> 3)) >> 4 * (yr & 7) << 4 * e;
+        if (DROP && SWAP) drops = drop_marks(a.p.mask, xr + e + a.p.row0, (unsigned)((yr + a.p.col0) >> 3)) >> 4 * (yr & 7) << 4 * e;
         if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * a.p.kept;
         out[e] = (T)v;
       }
@@ -440,11 +456,14 @@ inline bool launch_tiles(const MatmulArgs& a, int type, bool drop, hipStream_t s
 template <typename T, bool DROP, int FY, int FX, int W>
 inline void launch_few_as(const FewArgs& a, bool swap, hipStream_t st) {
   auto f = swap ? matmul_few<T, DROP, FY, FX, W, true> : matmul_few<T, DROP, FY, FX, W, false>;
-  hipLaunchKernelGGL(f, dim3((unsigned)((a.rows + 16 * FX - 1) / (16 * FX))), dim3(64 * W), 0, st, a);
+  hipLaunchKernelGGL(f, dim3((unsigned)((a.rows + 16 * FX - 1) / (16 * FX)), (unsigned)((a.few + 16 * FY - 1) / (16 * FY))),
+                     dim3(64 * W), 0, st, a);
 }
 template <typename T, bool DROP>
-inline void launch_few(const FewArgs& a, bool swap, int cus, hipStream_t st) {
-  const int fy = (a.few + 15) / 16;
+inline void launch_few(const FewArgs& a, bool swap, int cus, int squares, hipStream_t st) {
+  if (squares == 1) return launch_few_as<T, DROP, 2, 2, 8>(a, swap, st);
+  if (squares == 2) return launch_few_as<T, DROP, 4, 2, 4>(a, swap, st);
+  const int64_t fy = (a.few + 15) / 16;
   const int64_t pieces = (a.rows + 15) / 16;
   if (fy == 1) {
     // few workgroups: more waves of each share k (1 x 256 x 16384 9.7 us)
@@ -468,7 +487,9 @@ inline bool few_rows(const MatmulArgs& p, int cus) {
   const int64_t few = std::min(p.m, p.n), many = std::max(p.m, p.n);
   return few <= 32 || (few <= 64 && many < (int64_t)cus * 64);
 }
-inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, hipStream_t st) {
+constexpr int64_t kMostFewRows = (int64_t)0x7fffff * 16;
+// squares: 0 for few rows on one side; 1, 2: a small product in pieces of 32 x 32 or 64 x 32.
+inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, int squares, hipStream_t st) {
   const bool swap = p.n < p.m;  // few columns of C: the rows of A are the many
   FewArgs a;
   a.p = p;
@@ -481,20 +502,90 @@ inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, h
   a.ldsx = swap ? p.ldsa : p.ldsb;
   a.ldsy = swap ? p.ldsb : p.ldsa;
   a.rows = swap ? p.m : p.n;
-  a.few = (int)(swap ? p.n : p.m);
-  if (a.rows > (int64_t)0x7fffff * 16) return false;
-  if (type == 0) drop ? launch_few<float, true>(a, swap, cus, st) : launch_few<float, false>(a, swap, cus, st);
-  else if (type == 1) drop ? launch_few<__bf16, true>(a, swap, cus, st) : launch_few<__bf16, false>(a, swap, cus, st);
-  else drop ? launch_few<_Float16, true>(a, swap, cus, st) : launch_few<_Float16, false>(a, swap, cus, st);
+  a.few = swap ? p.n : p.m;
+  if (a.rows > kMostFewRows || a.few > 65535 * 16) return false;
+  if (type == 0) drop ? launch_few<float, true>(a, swap, cus, squares, st) : launch_few<float, false>(a, swap, cus, squares, st);
+  else if (type == 1) drop ? launch_few<__bf16, true>(a, swap, cus, squares, st) : launch_few<__bf16, false>(a, swap, cus, squares, st);
+  else drop ? launch_few<_Float16, true>(a, swap, cus, squares, st) : launch_few<_Float16, false>(a, swap, cus, squares, st);
   return true;
+}
+
+// How a product is cut up, by the microseconds each way is expected to take; constants from timing
+// all of them over sizes from 256 x 256 x 16384 to 16384 x 8192 x 4096 on an idle device of 256
+// compute units (a launch alone counts 5).  S: steps of 128 along k.
+//   tiles of 256 x 256, one to a compute unit at a time    12 + 0.89 S a round   (8192^3: 279 us)
+//   tiles of 128 x 256                                     7.6 + 0.57 S a round  (8192^3: 352)
+//   tiles of 128 x 128, two to a compute unit              3.4 + 0.74 S a round  (8192^3: 403)
+//                       no more than compute units         3 + 0.27 S
+//   64 x 32 and 32 x 32 pieces straight from memory: what they load over and over, or one wave's
+//   share of k                          (512 x 512 x 8192: 19 and 14 us, tiles of 128 x 128 22)
+enum Cut { kTiles256, kTiles128x256, kTiles128, kPieces64, kPieces32 };
+struct Plan {
+  Cut cut;
+  double us;
+};
+inline Plan plan_matmul(int64_t m, int64_t n, int chunks, int cus) {
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+  auto rounds = [&](int64_t t, int64_t at_once) { return (double)((t + at_once - 1) / at_once); };
+  const double s = chunks, work = (double)m * (double)n * 128. * s;
+  const int64_t small = tiles(128, 128);
+  const Plan ways[] = {
+      {kTiles256, 5 + rounds(tiles(256, 256), cus) * (12 + 0.89 * s)},
+      {kTiles128x256, 5 + rounds(tiles(128, 256), cus) * (7.6 + 0.57 * s)},
+      {kTiles128, small <= cus ? 8 + 0.27 * s : 6 + rounds(small, 2 * cus) * (3.4 + 0.74 * s)},
+      {kPieces64, 5 + std::max(3.6e-9 * work, 0.22 * s)},
+      {kPieces32, 5 + std::max(5e-9 * work, 0.13 * s)}};
+  Plan best = ways[0];
+  for (const Plan& w : ways)
+    if (w.us < best.us) best = w;
+  return best;
 }
 
 // type: 0 float, 1 bfloat16, 2 half.  False when the grid would not fit one launch.
 inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hipStream_t st) {
-  if (few_rows(a, cus)) return launch_few_rows(a, type, drop, cus, st);
-  const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-  if (big >= cus / 2) return launch_tiles<256, 256, 128, 64>(a, type, drop, st);
-  return launch_tiles<128, 128, 64, 64>(a, type, drop, st);
+  if (few_rows(a, cus)) return launch_few_rows(a, type, drop, cus, 0, st);
+  const Plan whole = plan_matmul(a.m, a.n, a.chunks, cus);
+  // A few rows or columns over a multiple of 256 can cost a round of tiles of their own: they go to
+  // the kernel for few rows, in a launch of theirs (4096 x 4100 x 2048: 39 us whole, 33 cut).
+  const int64_t over_m = a.m % 256 <= 64 ? a.m % 256 : 0, over_n = a.n % 256 <= 64 ? a.n % 256 : 0;
+  if (whole.cut <= kTiles128 && (over_m || over_n) && a.m > 256 && a.n > 256 && std::max(a.m, a.n) <= kMostFewRows) {
+    const double cost = plan_matmul(a.m - over_m, a.n - over_n, a.chunks, cus).us +
+                        (over_m ? 7 : 0) + (over_n ? 7 : 0);
+    if (cost < whole.us) {
+      const int64_t size = type == 0 ? 4 : 2;
+      MatmulArgs in = a;
+      in.m -= over_m;
+      in.n -= over_n;
+      if (!launch_matmul(in, type, drop, cus, st)) return false;
+      if (over_n) {  // columns at the right, all rows
+        MatmulArgs r = a;
+        r.n = over_n;
+        r.b += in.n * a.ldb;
+        r.sb += in.n * a.ldsb;
+        r.c = static_cast<char*>(a.c) + in.n * size;
+        r.col0 += in.n;
+        if (!launch_few_rows(r, type, drop, cus, 0, st)) return false;
+      }
+      if (over_m) {  // rows at the bottom, the columns that are left
+        MatmulArgs r = a;
+        r.m = over_m;
+        r.n = in.n;
+        r.a += in.m * a.lda;
+        r.sa += in.m * a.ldsa;
+        r.c = static_cast<char*>(a.c) + in.m * a.ldc * size;
+        r.row0 += in.m;
+        if (!launch_few_rows(r, type, drop, cus, 0, st)) return false;
+      }
+      return true;
+    }
+  }
+  switch (whole.cut) {
+    case kTiles256: return launch_tiles<256, 256, 128, 64>(a, type, drop, st);
+    case kTiles128x256: return launch_tiles<128, 256, 64, 64>(a, type, drop, st);
+    case kTiles128: return launch_tiles<128, 128, 64, 64>(a, type, drop, st);
+    case kPieces64: return launch_few_rows(a, type, drop, cus, 2, st);
+    default: return launch_few_rows(a, type, drop, cus, 1, st);
+  }
 }
 
 }  // namespace plr_mx

@@ -186,7 +186,8 @@ MATMULS = [(1, 1, 1), (1, 1, 128), (1, 300, 1000), (2, 17, 129), (3, 64, 2048), 
            (128, 256, 1000), (255, 257, 384), (300, 520, 777), (512, 512, 1024), (1, 5000, 8192),
            (1000, 1, 300), (7, 9, 16500), (256, 768, 640), (513, 1025, 2100),
            (4100, 2200, 300), (2049, 4097, 129), (5000, 20, 300), (40, 9000, 260),
-           (50, 8200, 640), (20000, 50, 513), (64, 64, 128), (17, 4000, 2000)]
+           (50, 8200, 640), (20000, 50, 513), (64, 64, 128), (17, 4000, 2000),
+           (4100, 4100, 200), (4097, 3900, 300), (1100, 2300, 500), (70, 4000, 1000), (500, 500, 4000)]
 
 
 def _matmul(capi, a, b, k, dtype, alpha=1.0, drop=None, pad=0, ldc=None, poison=77.0, more=0):

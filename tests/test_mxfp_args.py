@@ -124,7 +124,8 @@ def test_dequantize_refusals(capi, change, what):
     (dict(ldsa=6), "scale pitches"), (dict(ldsb=2), "scale pitches"), (dict(ldc=6), "ldc"),
     (dict(da=None), "NULL"), (dict(dsb=None), "NULL"), (dict(dc=None), "NULL"),
     (dict(da=P + 8), "16-byte"), (dict(dsa=P + 2), "4-byte"), (dict(dc=P + 2), "element type"),
-    (dict(m=1 << 40), "2^31"), (dict(lda=1 << 62), "too large"),
+    (dict(m=1 << 40), "2^31"), (dict(lda=1 << 62), "2^23"), (dict(k=(1 << 24) + 1), "2^24"),
+    (dict(ldsb=1 << 24), "2^23"), (dict(ldc=1 << 62), "too large"),
 ])
 def test_matmul_refusals(capi, change, what):
     a = dict(m=5, n=7, k=100, da=P, lda=64, dsa=P, ldsa=4, db=P, ldb=64, dsb=P, ldsb=4, dc=P, dtype=1,
@@ -134,14 +135,9 @@ def test_matmul_refusals(capi, change, what):
 
 
 def test_matmul_workspace_is_asked_for(capi):
-    big = [(m, n, k) for m in (1, 16, 100) for n in (1, 64, 4096) for k in (128, 16384)
-           if capi.mxfp_matmul_workspace(m, n, k) > 0]
-    for m, n, k in big:
-        p, q = capi.mxfp_code_pitch(k), capi.mxfp_scale_pitch(k)
-        size = capi.mxfp_matmul_workspace(m, n, k)
-        for space, have in ((None, size), (P, size - 1), (P + 8, size)):
-            refused("workspace", capi.mxfp_matmul, m, n, k, P, p, P, q, P, p, P, q, P, 1, n,
-                    workspace=space, workspace_bytes=have)
+    assert [capi.mxfp_matmul_workspace(m, n, k) for m, n, k in ((1, 1, 1), (100, 4096, 16384))] == [0, 0]
+    refused("workspace", capi.mxfp_matmul, 5, 7, 100, P, 64, P, 4, P, 64, P, 4, P, 1, 7,
+            workspace=P, workspace_bytes=-1)
 
 
 def test_context_calls_refuse_null(capi):
