@@ -95,6 +95,69 @@ __device__ __forceinline__ void store_pack(T* p, int64_t c, int64_t cols, const 
   }
 }
 
+// How the 32 columns of a block lie over a quad's lanes: lane l takes P pieces of V = 16 bytes'
+// worth of columns, piece i from column 32 / P * i + V * l on, so that a quad's load or store is 64
+// consecutive bytes for every type (with 8 consecutive columns to a lane the 250000 x 512 doubles
+// below took 247 us to codes, 250000 x 512 floats 141 us back).
+template <typename T>
+struct Piece {
+  static constexpr int V = 16 / (int)sizeof(T), P = 8 / V;
+  static __device__ __forceinline__ int column(int i, int l) { return 32 / P * i + V * l; }
+};
+template <int A, int B, int C, int D>
+__device__ __forceinline__ unsigned quad_perm(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, A | B << 2 | C << 4 | D << 6, 0xf, 0xf, true);
+}
+// Four codewords of a quad, byte b of lane l's to byte l of lane b's.
+__device__ __forceinline__ unsigned quad_transpose(unsigned w, int l) {
+  unsigned o = quad_perm<1, 0, 3, 2>(w);
+  w = __builtin_amdgcn_perm(o, w, l & 1 ? 0x03070105u : 0x06020400u);
+  o = quad_perm<2, 3, 0, 1>(w);
+  return __builtin_amdgcn_perm(o, w, l & 2 ? 0x03020706u : 0x05040100u);
+}
+// A lane's 8 codes in the order of its pieces -> the codes of columns 8 l .. 8 l + 7, and back.
+template <typename T>
+__device__ __forceinline__ unsigned codes_in_order(unsigned w, int l) {
+  if constexpr (Piece<T>::P == 1) return w;
+  if constexpr (Piece<T>::P == 4) return quad_transpose(w, l);
+  return __builtin_amdgcn_perm(quad_perm<1, 3, 1, 3>(w), quad_perm<0, 2, 0, 2>(w), l & 2 ? 0x07060302u : 0x05040100u);
+}
+template <typename T>
+__device__ __forceinline__ unsigned codes_of_pieces(unsigned w, int l) {
+  if constexpr (Piece<T>::P == 1) return w;
+  if constexpr (Piece<T>::P == 4) return quad_transpose(w, l);
+  return __builtin_amdgcn_perm(quad_perm<2, 2, 3, 3>(w), quad_perm<0, 0, 1, 1>(w), l & 1 ? 0x07060302u : 0x05040100u);
+}
+// The marks of columns 8 l .. 8 l + 7 (four bits each) -> those of the lane's pieces.
+template <typename T>
+__device__ __forceinline__ unsigned marks_of_pieces(unsigned m, int l) {
+  if constexpr (Piece<T>::P == 1) return m;
+  if constexpr (Piece<T>::P == 2)
+    return (quad_perm<0, 0, 1, 1>(m) >> 16 * (l & 1) & 0xffffu) | quad_perm<2, 2, 3, 3>(m) >> 16 * (l & 1) << 16;
+  return quad_transpose(m, l);
+}
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> load_pieces(const T* row, int64_t block, int l, int64_t cols) {
+  Pack<T, 8> r;
+#pragma unroll
+  for (int i = 0; i < Piece<T>::P; ++i) {
+    const auto p = load_pack<T, Piece<T>::V>(row, block + Piece<T>::column(i, l), cols);
+#pragma unroll
+    for (int e = 0; e < Piece<T>::V; ++e) r.v[Piece<T>::V * i + e] = p.v[e];
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_pieces(T* row, int64_t block, int l, int64_t cols, const Pack<T, 8>& r) {
+#pragma unroll
+  for (int i = 0; i < Piece<T>::P; ++i) {
+    Pack<T, Piece<T>::V> p;
+#pragma unroll
+    for (int e = 0; e < Piece<T>::V; ++e) p.v[e] = r.v[Piece<T>::V * i + e];
+    store_pack<T, Piece<T>::V>(row, block + Piece<T>::column(i, l), cols, p);
+  }
+}
+
 // ---------------------------------------------------------------- quantisation
 // The bits of |v| that order magnitudes and hold the exponent: for doubles the high word.
 __device__ __forceinline__ unsigned mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -191,7 +254,17 @@ struct QuantArgs {
 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantRows = 4;  // row sets per workgroup: as many loads in flight per thread
+// row sets per workgroup: few stores to a thread keep more of them going at once (250000 x 512
+// floats to codes and back: 99 + 120 us with one set, 106 + 142 with four), but the mask's first
+// rounds and narrow loads want a few (16385 x 4100 bfloat16: 28 and 28 us with three and two, 32 and
+// 28 with one)
+template <typename T>
+constexpr int kQuantRows = sizeof(T) == 2 ? 3 : 1;
+template <typename T>
+constexpr int kMoveRows = sizeof(T) == 2 ? 2 : 1;
+// waves of a workgroup of quantize_columns, side by side along the rows of x: unaligned rows have
+// lines that two of them read (16385 x 4100 bfloat16: 49 us with one, 38 with four, 42 with eight)
+constexpr int kColumnWaves = 4;  // row sets per workgroup: as many loads in flight per thread
 
 // Largest of the four lanes of a quad, in all four.
 __device__ __forceinline__ unsigned quad_max(unsigned v) {
@@ -210,18 +283,19 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
   const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
   const int rows = 16 >> a.tc_log2;  // rows per set
-  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
-  const int64_t c = chunk * 128 + l16 * 8;
+  const int64_t row = (int64_t)by * rows * kQuantRows<T> + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8, block = c & ~31;
+  const int l4 = l16 & 3;
   const T* x = static_cast<const T*>(a.x);
   const MaskGroup group = DROP ? mask_group(a.mask, (unsigned)(c >> 3)) : MaskGroup{};
-  Pack<T, 8> in[kQuantRows];
+  Pack<T, 8> in[kQuantRows<T>];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kQuantRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
-    if (r < a.n) in[u] = load_pack<T, 8>(x + r * a.ldx, c, a.d);
+    if (r < a.n) in[u] = load_pieces<T>(x + r * a.ldx, block, l4, a.d);
   }
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kQuantRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;  // (a quad shares its row: its lanes leave together)
     unsigned top = 0, s, w;
@@ -240,7 +314,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
       w = s == 255u ? 0u : encode_pairs<T>(pairs, scale_value(s));
     } else {
     W v[8];
-    const unsigned drop = DROP ? drop_marks(a.mask, group, mask_row(a.mask, r)) : 0u;
+    const unsigned drop = DROP ? marks_of_pieces<T>(drop_marks(a.mask, group, mask_row(a.mask, r)), l4) : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = Elem<T>::up(in[u].v[i]);
@@ -249,7 +323,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
       top = b > top ? b : top;
     }
     s = scale_byte(quad_max(top), W(0));
-    w = s == 255u ? 0u : encode8(v, s);
+    w = codes_in_order<T>(s == 255u ? 0u : encode8(v, s), l4);
     }
     if (c / 2 < a.ldc && chunk < a.chunks)
       *reinterpret_cast<unsigned*>(a.codes + r * a.ldc + c / 2) = w;
@@ -286,19 +360,21 @@ __device__ __forceinline__ void put_column_block(const QuantArgs& a, const Pack<
 // Blocks along a column: row j of the result is column j of x.  A thread holds V = 16 bytes of
 // columns times 32 rows in registers -- so a block never leaves its thread --, 8 lanes cover 128
 // bytes of a row of x and the 8 groups of lanes 256 rows, so that a result row is written in
-// pieces of 128 bytes.  The columns behind the last whole V are left to workgroups of their own
-// (the last of a tile row), where a thread takes one column.
+// pieces of 128 bytes.  The columns behind the last whole V are left to a wave of their own (the
+// last of a tile row), where a thread takes one column.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(64, 2) void quantize_columns(QuantArgs a) {
+__global__ __launch_bounds__(64 * kColumnWaves, 2) void quantize_columns(QuantArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
-  const unsigned by = blockIdx.x / a.nbx, bx = blockIdx.x - by * a.nbx;
-  const int lane = threadIdx.x;
+  const unsigned by = blockIdx.x / a.nbx;
+  const unsigned bx = (blockIdx.x - by * a.nbx) * kColumnWaves + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int64_t blk = (int64_t)by * 8 + (lane >> 3);  // block of 32 rows
   const int64_t r0 = blk * 32;
   const int64_t whole = a.d / V * V;
   if (blk * 16 >= a.ldc || blk >= a.chunks * 4) return;
   const T* x = static_cast<const T*>(a.x);
   if ((int64_t)bx * 8 * V >= whole) {
+    if ((int64_t)bx * 8 * V >= whole + 8 * V) return;  // one wave for what is over
     const int64_t c = whole + (lane & 7);
     if (c >= a.d) return;
     const MaskGroup group = DROP ? mask_group(a.mask, (unsigned)(c >> 3)) : MaskGroup{};
@@ -404,12 +480,13 @@ __global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) 
   const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
   const int rows = 16 >> a.tc_log2;
-  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
-  const int64_t c = chunk * 128 + l16 * 8;
-  if (c >= a.d) return;
-  unsigned w[kQuantRows], s[kQuantRows];
+  const int64_t row = (int64_t)by * rows * kMoveRows<T> + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8, block = c & ~31;
+  const int l4 = l16 & 3;
+  if (block >= a.d) return;  // (a quad's lanes stay together; a started block has all its codes)
+  unsigned w[kMoveRows<T>], s[kMoveRows<T>];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kMoveRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r < a.n) {
       w[u] = *reinterpret_cast<const unsigned*>(a.codes + r * a.ldc + c / 2);
@@ -417,17 +494,18 @@ __global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) 
     }
   }
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kMoveRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;
     // the product with the scale is exact in the wide type unless it leaves its range
-    const v2f q[4] = {decode2<0>(w[u]), decode2<1>(w[u]), decode2<2>(w[u]), decode2<3>(w[u])};
+    const unsigned wp = codes_of_pieces<T>(w[u], l4);
+    const v2f q[4] = {decode2<0>(wp), decode2<1>(wp), decode2<2>(wp), decode2<3>(wp)};
     const W sc = s[u] == 255u ? W(__builtin_nanf("")) : sizeof(W) == 8 ? W(scale_value_f64(s[u]))
                                                                        : W(scale_value(s[u]));
     Pack<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = Elem<T>::down((W)q[i >> 1][i & 1] * sc);
-    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, o);
+    store_pieces<T>(static_cast<T*>(a.out) + r * a.ldo, block, l4, a.d, o);
   }
 }
 
@@ -450,27 +528,28 @@ __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
   const int slot = threadIdx.x >> 4, l16 = threadIdx.x & 15;
   const int64_t chunk = ((int64_t)bx << a.tc_log2) + (slot & ((1 << a.tc_log2) - 1));
   const int rows = 16 >> a.tc_log2;
-  const int64_t row = (int64_t)by * rows * kQuantRows + (slot >> a.tc_log2);
-  const int64_t c = chunk * 128 + l16 * 8;
-  if (c >= a.d) return;
-  Pack<T, 8> in[kQuantRows];
+  const int64_t row = (int64_t)by * rows * kMoveRows<T> + (slot >> a.tc_log2);
+  const int64_t c = chunk * 128 + l16 * 8, block = c & ~31;
+  const int l4 = l16 & 3;
+  if (block >= a.d) return;  // (a quad's lanes stay together)
+  Pack<T, 8> in[kMoveRows<T>];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kMoveRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
-    if (r < a.n) in[u] = load_pack<T, 8>(static_cast<const T*>(a.x) + r * a.ldx, c, a.d);
+    if (r < a.n) in[u] = load_pieces<T>(static_cast<const T*>(a.x) + r * a.ldx, block, l4, a.d);
   }
   const W sc = (W)a.scale;
   const MaskGroup group = mask_group(a.mask, (unsigned)(c >> 3));
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kMoveRows<T>; ++u) {
     const int64_t r = row + (int64_t)u * rows;
     if (r >= a.n) continue;
-    const unsigned drop = drop_marks(a.mask, group, mask_row(a.mask, r));
+    const unsigned drop = marks_of_pieces<T>(drop_marks(a.mask, group, mask_row(a.mask, r)), l4);
     Pack<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       o.v[i] = (drop >> 4 * i & 1) ? T(0) : Elem<T>::down(Elem<T>::up(in[u].v[i]) * sc);
-    store_pack<T, 8>(static_cast<T*>(a.out) + r * a.ldo, c, a.d, o);
+    store_pieces<T>(static_cast<T*>(a.out) + r * a.ldo, block, l4, a.d, o);
   }
 }
 
@@ -580,9 +659,9 @@ bool fits_launch(int64_t x, int64_t y, int threads) {
 }
 
 // Workgroups of the tiled kernels; false when a launch cannot hold them.
-bool tile_grid(int64_t n, int64_t chunks, int tc, unsigned* nbx, unsigned* grid) {
+bool tile_grid(int64_t n, int64_t chunks, int tc, int sets, unsigned* nbx, unsigned* grid) {
   const int64_t x = ceil_div(chunks, (int64_t)1 << tc);
-  const int64_t y = ceil_div(n, (int64_t)(16 >> tc) * kQuantRows);
+  const int64_t y = ceil_div(n, (int64_t)(16 >> tc) * sets);
   if (!fits_launch(x, y, kQuantThreads)) return false;
   *nbx = (unsigned)x;
   *grid = (unsigned)(x * y);
@@ -593,7 +672,7 @@ template <typename T>
 void launch_quantize(const QuantArgs& a, bool transpose, bool drop, unsigned grid, hipStream_t st) {
   if (transpose) {
     auto f = drop ? quantize_columns<T, true> : quantize_columns<T, false>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(64), 0, st, a);
+    hipLaunchKernelGGL(f, dim3(grid), dim3(64 * kColumnWaves), 0, st, a);
   } else {
     auto f = drop ? quantize_rows<T, true> : quantize_rows<T, false>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(kQuantThreads), 0, st, a);
@@ -650,13 +729,13 @@ int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned 
   unsigned grid = 0;
   if (tr) {
     const int64_t v = 16 / (int64_t)size;  // columns a thread takes; what is over has its own workgroups
-    const int64_t x = ceil_div(d / v, 8) + (d % v != 0), y = ceil_div(a.chunks * 4, 8);
-    if (!fits_launch(x, y, 64)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
+    const int64_t x = ceil_div(ceil_div(d / v, 8) + (d % v != 0), kColumnWaves), y = ceil_div(a.chunks * 4, 8);
+    if (!fits_launch(x, y, 64 * kColumnWaves)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
     a.nbx = (unsigned)x;
     grid = (unsigned)(x * y);
   } else {
     a.tc_log2 = tile_log2(a.chunks);
-    if (!tile_grid(n, a.chunks, a.tc_log2, &a.nbx, &grid))
+    if (!tile_grid(n, a.chunks, a.tc_log2, size == 2 ? kQuantRows<__bf16> : kQuantRows<float>, &a.nbx, &grid))
       return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   }
   rc = c.begin(device_id, hip_stream);
@@ -702,7 +781,7 @@ int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, 
   const int64_t chunks = ceil_div(d, 128);
   a.tc_log2 = tile_log2(chunks);
   unsigned grid = 0;
-  if (!tile_grid(n, chunks, a.tc_log2, &a.nbx, &grid))
+  if (!tile_grid(n, chunks, a.tc_log2, size == 2 ? kMoveRows<__bf16> : kMoveRows<float>, &a.nbx, &grid))
     return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   int rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || n == 0) return rc;
@@ -742,7 +821,7 @@ int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned 
   const int64_t chunks = ceil_div(d, 128);
   a.tc_log2 = tile_log2(chunks);
   unsigned grid = 0;
-  if (!tile_grid(n, chunks, a.tc_log2, &a.nbx, &grid))
+  if (!tile_grid(n, chunks, a.tc_log2, size == 2 ? kMoveRows<__bf16> : kMoveRows<float>, &a.nbx, &grid))
     return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || n == 0) return rc;
