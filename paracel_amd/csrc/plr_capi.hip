@@ -214,34 +214,50 @@ int g_na_occ[kNaMaxDevices][kNaMaxPitch / plr::kChunkCols + 1] = {};
 std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 
 // Shard held in 4 bits.  A row of up to kPackedFused blocks is read once (theta and the partial
-// dot products of two tiles have to fit a compute unit's LDS); wider ones go in column pieces of
-// kPackedPiece blocks, in two sweeps.
+// dot products of two tiles have to fit a compute unit's LDS); wider ones go in column pieces, in
+// two sweeps.
 typedef void (*packed_fn)(plr::PackedArgs);
 struct PackedFns {
-  int stride;         // blocks of theta in LDS: the widest row
+  int stride;         // blocks of theta in LDS (none: 0): the widest row or piece
   int sets;           // row sets of a tile
   int threads;
-  packed_fn grad[2];  // [dropout]
-  packed_fn eval;
+  int most_slots;     // rows side by side
+  packed_fn fn;
+};
+enum { kGrad, kGradDrop, kEval };
+struct PackedFused {
+  PackedFns fns[3];
 };
 template <int STRIDE, int SR, int NT, int MINW>
-constexpr PackedFns make_packed() {
-  return {STRIDE, SR, NT,
-          {plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>,
-           plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
-          plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>};
+constexpr PackedFused make_packed() {
+  return {{{STRIDE, SR, NT, NT, plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>},
+           {STRIDE, SR, NT, NT, plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
+           {STRIDE, SR, NT, NT, plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>}}};
 }
 // Row sets per tile: as many as leave two workgroups (of 512 threads one) on a compute unit; the
 // barriers and row terms of a tile cost the same however long it is (1M x 1000: 16 sets 265 us,
 // 8 sets 301).  Rows of up to 8 blocks lie 32 and more side by side: with 8 sets their partials
 // stay small enough (1M x 100 with dropout: 8 sets 80 us, 16 sets 92).
-const PackedFns kPacked[4] = {make_packed<8, 8, 256, 2>(), make_packed<64, 16, 256, 2>(),
+const PackedFused kPacked[4] = {make_packed<8, 8, 256, 2>(), make_packed<64, 16, 256, 2>(),
                               make_packed<256, 8, 512, 2>(), make_packed<512, 4, 512, 2>()};
-const packed_fn kPackedDot[2] = {plr::packed_pass<false, false, plr::kPassDot, 256, 8, 512, 2>,
-                                 plr::packed_pass<false, true, plr::kPassDot, 256, 8, 512, 2>};
-const packed_fn kPackedAxpy[2] = {plr::packed_pass<true, false, plr::kPassAxpy, 256, 8, 512, 2>,
-                                  plr::packed_pass<true, true, plr::kPassAxpy, 256, 8, 512, 2>};
-constexpr int kPackedFused = 480, kPackedPiece = 256;
+// The sweeps wait for memory more than they compute: as many waves as their registers allow, in the
+// second one side by side in one workgroup, whose sums then leave it as one (12000 x 16385: three
+// workgroups of 256 threads 81 us a pass, one of 768 79; 3000 x 40001: 72 and 57).
+constexpr int kPackedFused = 480, kDotPiece = 128, kAxpyPiece = 256, kSweepSlots = 64;
+struct PackedSweep {
+  int most_blocks;  // of a piece
+  PackedFns fns[2];  // [dropout]
+};
+template <int SR, int NT, int MINW, bool DROP>
+constexpr PackedFns make_dot() {
+  return {kDotPiece, SR, NT, kSweepSlots, plr::packed_pass<false, DROP, plr::kPassDot, kDotPiece, SR, NT, MINW>};
+}
+template <int SR, int NT, int MINW, bool DROP>
+constexpr PackedFns make_axpy() {
+  return {0, SR, NT, kSweepSlots, plr::packed_pass<true, DROP, plr::kPassAxpy, 0, SR, NT, MINW>};
+}
+const PackedSweep kDot = {kDotPiece, {make_dot<8, 512, 4, false>(), make_dot<8, 512, 2, true>()}};
+const PackedSweep kAxpy = {kAxpyPiece, {make_axpy<8, 768, 3, false>(), make_axpy<8, 512, 2, true>()}};
 
 }  // namespace
 
@@ -253,6 +269,13 @@ int plr_fail_without_context(int code, const char* msg) {
   }
   return code;
 }
+
+struct PackedLaunch {
+  const PackedFns* fns = nullptr;
+  int64_t piece = 0, steps = 0;  // blocks; groups of row sets per workgroup
+  int pieces = 0, grid = 0;
+  size_t lds = 0;
+};
 
 struct plr_ctx {
   int device = 0;
@@ -348,8 +371,8 @@ struct plr_ctx {
   uint8_t* d_codes = nullptr;     // n x row_blocks * 16 bytes
   uint8_t* d_scales = nullptr;    // n x row_blocks
   int64_t row_blocks = 0;
-  const PackedFns* packed_fns = nullptr;
-  int packed_grid[3] = {0, 0, 0};  // a gradient, one with dropout, none
+  PackedLaunch packed_plan[3];    // a gradient, one with dropout, none
+  PackedLaunch packed_dot[2];     // two sweeps: the first
   bool packed_sweeps = false;     // too wide for one read: column pieces, two sweeps
   bool drop_on = false;           // plr_set_dropout
   plr_dropout drop = {0., 0, 0, 0};
@@ -611,38 +634,60 @@ int plan_shape(plr_ctx* c, int64_t n, int64_t d) {
   return PLR_OK;
 }
 
-// Rows side by side.  (A narrow last piece of a wide row does not need every thread, and what is
-// read behind the last row stays short.)
-int packed_slots(const PackedFns* f, int blocks) {
-  return std::min(f->threads / blocks, f->stride == kPackedPiece ? 64 : f->threads);
+int packed_slots(const PackedFns* f, int64_t blocks) {
+  return (int)std::min<int64_t>(f->threads / blocks, f->most_slots);
 }
 
-// LDS: theta, partial dot products, residuals and (with dropout) marks of a tile, and in the end
-// 9 doubles a thread; of a row's widest and narrowest piece.
-size_t packed_lds(const PackedFns* f, int64_t row_blocks, bool drop) {
+// LDS: theta, partial dot products, residuals and (with dropout, between the halves of a fused
+// pass) marks of a tile, and in the end 9 doubles a thread; of a row's widest and narrowest piece.
+size_t packed_lds(const PackedFns* f, int64_t row_blocks, int64_t piece, bool marks) {
   auto one = [&](int64_t blocks) {
-    const size_t rows = (size_t)packed_slots(f, (int)blocks) * f->sets;
+    const size_t rows = f->stride ? (size_t)packed_slots(f, blocks) * f->sets : 0;
     return std::max((size_t)f->threads * 9, (size_t)32 * f->stride + rows * ((blocks | 1) + 1)) * sizeof(double) +
-           (drop ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
+           (marks ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
   };
-  if (row_blocks <= kPackedFused) return one(row_blocks);
-  const int64_t over = row_blocks % kPackedPiece;
-  return std::max(one(kPackedPiece), over ? one(over) : 0);
+  const int64_t over = row_blocks % piece;
+  return std::max(one(std::min(piece, row_blocks)), over ? one(over) : 0);
 }
 
-const PackedFns* packed_fns_for(int64_t blocks) {
-  return &kPacked[blocks <= 8                                  ? 0
-                  : blocks <= 64                               ? 1
-                  : blocks <= 256 || blocks > kPackedFused ? 2
-                                                               : 3];
+const PackedFused& packed_fused_for(int64_t blocks) {
+  return kPacked[blocks <= 8 ? 0 : blocks <= 64 ? 1 : blocks <= 256 ? 2 : 3];
 }
 
 // Rows the kernels may read behind the last one: less than a group of row sets of any launch.
 int64_t packed_slack_rows(int64_t row_blocks) {
-  const PackedFns* f = packed_fns_for(row_blocks);
-  const int64_t least = row_blocks > kPackedFused && row_blocks % kPackedPiece
-                            ? row_blocks % kPackedPiece : std::min<int64_t>(row_blocks, kPackedPiece);
-  return (int64_t)packed_slots(f, (int)(row_blocks > kPackedFused ? least : row_blocks)) * plr::kPackedR;
+  return (int64_t)plr::kPackedR * (row_blocks > kPackedFused ? kSweepSlots
+                                                             : packed_slots(&packed_fused_for(row_blocks).fns[kGrad], row_blocks));
+}
+
+// One launch over n rows: its kernel, the blocks of a column piece and its persistent grid.
+int plan_packed_launch(plr_ctx* c, const PackedFns* f, int64_t n, int64_t piece, bool marks, PackedLaunch* l) {
+  const void* k = reinterpret_cast<const void*>(f->fn);
+  PLR_HIP(c, hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
+  l->fns = f;
+  l->piece = piece;
+  l->pieces = (int)ceil_div(c->row_blocks, piece);
+  l->lds = packed_lds(f, c->row_blocks, piece, marks);
+  int occ = 0;
+  PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k, f->threads, l->lds));
+  if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
+  const int64_t groups = ceil_div(n, (int64_t)packed_slots(f, piece) * plr::kPackedR);
+  l->grid = (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)c->num_cu * occ / l->pieces));
+  l->steps = ceil_div(groups, l->grid);
+  return PLR_OK;
+}
+
+// A sweep in pieces as even as may be, as many as leave a workgroup the fewest groups of row sets
+// (513 blocks in pieces of 256, 256 and 1 take a round of workgroups more than in 9 of 57).
+int plan_packed_sweep(plr_ctx* c, const PackedSweep& s, bool drop, int64_t n, PackedLaunch* best) {
+  const int64_t least = ceil_div(c->row_blocks, s.most_blocks);
+  for (int64_t pieces = least; pieces <= least + 8; ++pieces) {
+    PackedLaunch l;
+    const int rc = plan_packed_launch(c, &s.fns[drop], n, ceil_div(c->row_blocks, pieces), false, &l);
+    if (rc != PLR_OK) return rc;
+    if (pieces == least || l.steps < best->steps) *best = l;
+  }
+  return PLR_OK;
 }
 
 // Workgroup and persistent grid of the passes over n rows of dcols columns held in 4 bits.
@@ -652,41 +697,29 @@ int plan_packed(plr_ctx* c, int64_t n) {
   c->packed_sweeps = c->row_blocks > kPackedFused;
   c->var = &kBlockShape;  // unused by this path, kept non-null
   c->nch_rt = 1;
-  const int blocks = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
-  const PackedFns* pf = packed_fns_for(blocks);
-  c->packed_fns = pf;
-  const int64_t groups = ceil_div(n, (int64_t)packed_slots(pf, blocks) * plr::kPackedR);
-  // [without dropout, with it, without a gradient]: the instances that a pass of that kind launches
-  const packed_fn used[3][2] = {{pf->grad[0], pf->grad[0]}, {pf->grad[1], pf->grad[1]},
-                                {pf->eval, pf->eval}};
-  const packed_fn sweeps[3][2] = {{kPackedDot[0], kPackedAxpy[0]}, {kPackedDot[1], kPackedAxpy[1]},
-                                  {kPackedDot[0], kPackedDot[0]}};
-  for (int k = 0; k < 3; ++k) {
-    int occ = 1 << 30;
-    for (int i = 0; i < 2; ++i) {
-      const void* f = reinterpret_cast<const void*>(c->packed_sweeps ? sweeps[k][i] : used[k][i]);
-      PLR_HIP(c, hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512));
-      int o = 0;
-      PLR_HIP(c, hipOccupancyMaxActiveBlocksPerMultiprocessor(&o, f, pf->threads,
-                                                              packed_lds(pf, c->row_blocks, k == 1)));
-      occ = std::min(occ, o);
+  int rc = PLR_OK;
+  if (c->packed_sweeps) {
+    for (int k = 0; k < 2 && rc == PLR_OK; ++k) {
+      rc = plan_packed_sweep(c, kAxpy, k == 1, n, &c->packed_plan[k]);
+      if (rc == PLR_OK) rc = plan_packed_sweep(c, kDot, k == 1, n, &c->packed_dot[k]);
     }
-    if (occ < 1) return fail(c, PLR_ERR_HIP, "kernel variant does not fit on a compute unit");
-    // pieces side by side share the device: fewer, longer workgroups leave fewer partials to add up
-    // (12000 x 16385: 97 -> 88 us a pass)
-    const int64_t wide = c->packed_sweeps ? c->row_blocks / kPackedPiece : 1;
-    c->packed_grid[k] =
-        (int)std::max<int64_t>(1, std::min<int64_t>(groups, (int64_t)c->num_cu * occ / wide));
+    c->packed_plan[kEval] = c->packed_dot[0];
+  } else {
+    const PackedFused& f = packed_fused_for(c->row_blocks);
+    for (int k = kGrad; k <= kEval && rc == PLR_OK; ++k)
+      rc = plan_packed_launch(c, &f.fns[k], n, c->row_blocks, k == kGradDrop, &c->packed_plan[k]);
   }
-  c->grid = std::max(c->packed_grid[0], c->packed_grid[1]);
-  c->grid_nograd = c->packed_grid[2];
+  if (rc != PLR_OK) return rc;
+  const PackedLaunch &lg = c->packed_plan[kGrad], &ld = c->packed_plan[kGradDrop], &le = c->packed_plan[kEval];
+  c->grid = std::max(lg.grid, ld.grid);
+  c->grid_nograd = le.grid;
   char b[256];
   snprintf(b, sizeof b,
            "packed_pass<SR=%d> 4-bit shard, %lld blocks of 32 columns per row%s, %d rows side by side, "
            "grid=%d x %d threads (%d with dropout, %d without a gradient)",
-           pf->sets, (long long)c->row_blocks, c->packed_sweeps ? " in pieces of 256, two sweeps" : "",
-           packed_slots(pf, blocks), c->packed_grid[0], pf->threads, c->packed_grid[1],
-           c->packed_grid[2]);
+           lg.fns->sets, (long long)c->row_blocks, c->packed_sweeps ? " in pieces, two sweeps" : "",
+           packed_slots(lg.fns, lg.piece), lg.grid * lg.pieces, lg.fns->threads, ld.grid * ld.pieces,
+           le.grid * le.pieces);
   c->info = b;
   if (c->bias) c->info += "; first column constant 1, not stored";
   return PLR_OK;
@@ -766,7 +799,7 @@ int alloc_workspace(plr_ctx* c) {
     PLR_HIP(c, hipMalloc(&c->d_zparts, (size_t)c->zstride * c->nteams * c->team_blocks *
                                            plr::kTeamWaves * sizeof(double)));
   } else if ((c->blocked || c->packed_sweeps) && n > 0) {
-    const int64_t parts = c->packed_sweeps ? ceil_div(c->row_blocks, kPackedPiece) : 1;
+    const int64_t parts = c->packed_sweeps ? std::max(c->packed_dot[0].pieces, c->packed_dot[1].pieces) : 1;
     PLR_HIP(c, hipMalloc(&c->d_z, (size_t)n * parts * sizeof(double)));
     PLR_HIP(c, hipMalloc(&c->d_res, (size_t)n * sizeof(double)));
   }
@@ -845,6 +878,7 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
   a.pitch = c->pitch;
   a.loss_mode = pa.loss_mode;
   a.identity_link = pa.identity_link;
+  a.cols = c->dcols;
   a.kept = 1.;
   a.mask = plr_mx::Mask{0, 0, 0, 0, 0};
   const bool drop = grad && c->drop_on;
@@ -854,28 +888,25 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
     a.mask = plr_mx::Mask{t, (unsigned)c->drop.seed, (unsigned)(c->drop.seed >> 32),
                           c->drop.step + (unsigned)std::max(train_round, 0), c->drop.row0};
   }
-  const PackedFns* pf = c->packed_fns;
-  const int grid = c->packed_grid[!grad ? 2 : drop ? 1 : 0];
-  *parts = *loss_parts = grid;
-  a.piece = (int)(c->packed_sweeps ? kPackedPiece : c->row_blocks);
-  a.most_slots = packed_slots(pf, 1);
-  const int pieces = (int)ceil_div(c->row_blocks, a.piece);
-  const size_t lds = packed_lds(pf, c->row_blocks, drop);
-  auto launch = [&](packed_fn f) {
-    hipLaunchKernelGGL(f, dim3(grid, pieces), dim3(pf->threads), lds, c->stream, a);
+  auto launch = [&](const PackedLaunch& l) {
+    a.piece = (int)l.piece;
+    a.most_slots = l.fns->most_slots;
+    hipLaunchKernelGGL(l.fns->fn, dim3(l.grid, l.pieces), dim3(l.fns->threads), l.lds, c->stream, a);
     return hipGetLastError();
   };
+  const PackedLaunch& plan = c->packed_plan[!grad ? kEval : drop ? kGradDrop : kGrad];
+  *parts = *loss_parts = plan.grid;
   if (!c->packed_sweeps) {
-    PLR_HIP(c, launch(grad ? pf->grad[drop] : pf->eval));
+    PLR_HIP(c, launch(plan));
     return PLR_OK;
   }
-  PLR_HIP(c, launch(kPackedDot[drop]));
+  PLR_HIP(c, launch(c->packed_dot[drop]));
   hipLaunchKernelGGL(plr::packed_residual, dim3(c->res_grid), dim3(256), 0, c->stream, (const double*)c->d_z,
-                     pieces, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out, c->d_part_loss, c->n,
-                     pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res);
+                     c->packed_dot[drop].pieces, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
+                     c->d_part_loss, c->n, pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res);
   PLR_HIP(c, hipGetLastError());
   *loss_parts = c->res_grid;
-  if (grad) PLR_HIP(c, launch(kPackedAxpy[drop]));
+  if (grad) PLR_HIP(c, launch(plan));
   return PLR_OK;
 }
 

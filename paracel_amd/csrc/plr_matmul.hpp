@@ -72,8 +72,8 @@ __device__ __forceinline__ Out8<T> finish8(const MatmulArgs& p, int64_t i, int64
 
 // A wave's 16 x (16 FN) piece of C, rows i0 .., columns j0 ..; lane (r16, q) holds columns
 // 32 (y / 2) + 8 q .. + 7 of row r16 in acc[y], acc[y + 1] (y even).  Tiles that lie inside C are
-// stored as they are held; those at its edge go through 1 KB of LDS per wave and 32 columns, so that the code with the comparisons is there once and not for every
-// register.
+// stored as they are held; those at its edge go through 1 KB of LDS per
+// wave and 32 columns, so that the code with the comparisons is there once and not for every register.
 template <typename T, bool DROP, int FN>
 __device__ __forceinline__ void store_piece(const MatmulArgs& p, int64_t i0, int64_t j0, const v4f* acc, int r16,
                                             int q) {

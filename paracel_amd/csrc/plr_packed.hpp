@@ -42,7 +42,8 @@ struct PackedArgs {
   int64_t n;
   int64_t row_blocks;     // blocks of a stored row
   int64_t pitch;          // doubles per row of part_g
-  int piece;              // most blocks a workgroup takes; blockIdx.y is its piece of the row
+  int64_t cols;           // of the stored row
+  int piece;              // most blocks a workgroup takes; blockIdx.y counts pieces from the row's end
   int most_slots;         // most rows side by side
   unsigned loss_mode;
   int identity_link;
@@ -63,6 +64,7 @@ template <int R>
 struct PackedLoads {
   uint4 codes[R];
   unsigned char scales[R];
+  double res[R];  // kPassAxpy
 };
 template <int R>
 __device__ __forceinline__ PackedTile<R> arrived(const PackedLoads<R>& l) {
@@ -98,6 +100,14 @@ __device__ __forceinline__ double tile_scale(const PackedTile<R>& t, int r) {
 
 constexpr int kPackedR = 4;
 
+// The marks (bit q + 4 i: column 8 q + i) of a block's columns from `left` on.
+__device__ __forceinline__ unsigned columns_behind(int64_t left) {
+  unsigned m = 0;
+  for (int c = 0; c < 32; ++c)
+    if (c >= left) m |= 1u << ((c >> 3) + 4 * (c & 7));
+  return m;
+}
+
 // STRIDE: entries between theta's column pairs in LDS, at least `blocks` (fixed, so that a thread's
 // reads share one address).
 template <bool GRAD, bool DROP, int MODE, int STRIDE, int SR, int NT, int MINW>
@@ -106,7 +116,8 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
   static_assert(SR % R == 0, "whole groups of row sets");
   extern __shared__ double sm[];
   const int tid = threadIdx.x;
-  const int blk0 = (int)blockIdx.y * a.piece;
+  const int piece = (int)(gridDim.y - 1 - blockIdx.y);  // a narrow last one is not left to the end
+  const int blk0 = piece * a.piece;
   const int blocks = min(a.piece, (int)a.row_blocks - blk0);
   const int slots = min(NT / blocks, a.most_slots);
   const int max_rows = slots * SR;   // rows of a tile
@@ -140,7 +151,13 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
       const int64_t at = (set + r) * slots * a.row_blocks;  // the same for all threads
       t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
       t.scales[r] = (a.scales + at)[at_lane];
+      if (MODE == kPassAxpy) t.res[r] = a.res_in[min((set + r) * slots + slot, a.n - 1)];
     }
+  };
+  // A block that stands for NaN and is dropped whole is 0 all the same.
+  const unsigned behind = DROP ? columns_behind(a.cols - (int64_t)(blk0 + blk) * 32) : 0u;
+  auto nothing_kept = [&](PackedTile<R>& t, int r, unsigned marks) {
+    t.scales &= (marks | behind) == ~0u ? ~(255u << 8 * r) : ~0u;
   };
   // Zero what is dropped; marks[r]: bit q + 4 i is value 8 q + i of row r, 1 where dropped.
   auto drop = [&](int64_t set, PackedTile<R>& t, unsigned (&marks)[R]) {
@@ -156,6 +173,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
       t.codes[r].z &= plr_mx::kept_nibbles(m2);
       t.codes[r].w &= plr_mx::kept_nibbles(m3);
       marks[r] = m0 | m1 << 1 | m2 << 2 | m3 << 3;
+      nothing_kept(t, r, marks[r]);
     }
   };
   auto drop_again = [&](PackedTile<R>& t, int r, unsigned marks) {
@@ -163,6 +181,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
     t.codes[r].y &= plr_mx::kept_nibbles(marks >> 1 & 0x11111111u);
     t.codes[r].z &= plr_mx::kept_nibbles(marks >> 2 & 0x11111111u);
     t.codes[r].w &= plr_mx::kept_nibbles(marks >> 3 & 0x11111111u);
+    nothing_kept(t, r, marks);
   };
   auto update = [&](const PackedTile<R>& t, const double (&w)[R]) {
 #pragma unroll
@@ -248,7 +267,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
           if (row < a.n) {
             if (DROP) z *= a.kept;
             if (MODE == kPassDot) {
-              a.z_buf[(int64_t)blockIdx.y * a.n + row] = z;
+              a.z_buf[(int64_t)piece * a.n + row] = z;
             } else {
               double h, l;
               const double yv = a.y ? a.y[row] : 0.;
@@ -268,9 +287,13 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
 #pragma unroll 1
       for (int s = 0; s < sets; s += R) {
         PackedTile<R> cur = arrived(nxt);
+        double w[R];
+        if (MODE == kPassAxpy) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) w[r] = nxt.res[r];
+        }
         if (s + R < sets) load(set0 + s + R, nxt);
         else if (more) load(set0 + SR, nxt);
-        double w[R];
         if (MODE == kPassAxpy) {
           if (DROP) {
             unsigned marks[R];
@@ -279,7 +302,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const int64_t row = (set0 + s + r) * slots + slot;
-            w[r] = active && row < a.n ? a.res_in[row] * tile_scale(cur, r) : 0.;
+            w[r] = active && row < a.n ? w[r] * tile_scale(cur, r) : 0.;
           }
         } else {
 #pragma unroll

@@ -12,7 +12,7 @@ REL = 1e-11
 
 SHAPES = [(1, 1), (5, 2), (1000, 31), (777, 32), (64, 33), (5000, 41), (3000, 100), (1234, 257),
           (2500, 512), (1001, 1000), (999, 1100), (300, 2049), (257, 2080), (130, 4100), (67, 8193),
-          (40, 16384), (33, 16385), (21, 20000), (3, 40001), (1, 1000), (20000, 3)]
+          (40, 16384), (33, 16385), (21, 20000), (3, 40001), (1, 1000), (20000, 3), (700, 15361), (200, 30000)]
 
 
 def close(got, want, rel=REL):
@@ -194,6 +194,37 @@ def test_values_that_are_not_finite(plr):
     z = plr.predict_linear(theta)
     assert np.isnan(z[[11, 60]]).all() and np.isfinite(np.delete(z, [11, 60])).all()
     assert np.isnan(plr.loss_grad(theta)[1])
+
+
+@pytest.mark.parametrize("n, d", [(300, 38), (250, 70), (200, 1000), (150, 4100), (40, 16400), (30, 20001)])
+def test_a_nan_that_is_dropped_whole(plr, oracle, n, d):
+    # a block with a NaN stands for NaN, but where nothing of it is kept it counts 0 like any other
+    from paracel_amd import Dropout
+
+    X, y, theta = shard(n, d, 3)
+    drop = Dropout(0.97, 31, 1, 5)
+    keep = ref.keep(n, d, drop)
+    hit = 0
+    for i in range(n):
+        gone = [b for b in range(0, d, 32) if not keep[i, b:b + 32].any()]
+        if gone:
+            X[i, gone[i % len(gone)] if i % 3 else gone[-1]] = (np.nan, np.inf)[i % 2]
+            hit += 1
+    assert hit > n // 4
+    plr.set_data(X, y)
+    plr.pack_data()
+    plr.set_dropout(drop)
+    D = np.where(keep, ref.rounded(X), 0) * ref.kept_scale(0.97)
+    g, loss, _ = plr.loss_grad(theta, 3)
+    want, wl = expect(oracle, D, y, theta, 3)
+    close(g, want)
+    close(loss, wl)
+    # one that is kept makes the loss NaN
+    i, j = np.argwhere(keep)[len(np.argwhere(keep)) // 2]
+    X[i, j] = np.nan
+    plr.set_data(X, y)
+    plr.pack_data()
+    assert np.isnan(plr.loss_grad(theta, 3)[1])
 
 
 def test_rows_of_every_layout_pack_alike(plr):
