@@ -1943,7 +1943,7 @@ int plr_set_dropout(plr_ctx* c, const plr_dropout* drop) {
     if (drop->row0 < 0) return fail(c, PLR_ERR_INVALID, "dropout row0 must be >= 0");
     c->drop = *drop;
   }
-  c->drop_on = drop != nullptr;
+  c->drop_on = drop != nullptr && rint(drop->rate * 65536.) > 0.;
   return PLR_OK;
 }
 

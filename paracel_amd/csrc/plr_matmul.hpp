@@ -537,13 +537,13 @@ inline Plan plan_matmul(int64_t m, int64_t n, int chunks, int cus) {
       {kPieces32, 5 + std::max(5e-9 * work, 0.13 * s)}};
   Plan best = ways[0];
   for (const Plan& w : ways)
-    if (w.us < best.us) best = w;
+    if (w.us < best.us && (w.cut <= kTiles128 || std::max(m, n) <= kMostFewRows)) best = w;
   return best;
 }
 
 // type: 0 float, 1 bfloat16, 2 half.  False when the grid would not fit one launch.
 inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hipStream_t st) {
-  if (few_rows(a, cus)) return launch_few_rows(a, type, drop, cus, 0, st);
+  if (few_rows(a, cus) && std::max(a.m, a.n) <= kMostFewRows) return launch_few_rows(a, type, drop, cus, 0, st);
   const Plan whole = plan_matmul(a.m, a.n, a.chunks, cus);
   // A few rows or columns over a multiple of 256 can cost a round of tiles of their own: they go to
   // the kernel for few rows, in a launch of theirs (4096 x 4100 x 2048: 39 us whole, 33 cut).

@@ -50,7 +50,7 @@ __device__ __forceinline__ MaskGroup mask_group(const Mask& m, unsigned group) {
   return {(unsigned)(q >> 32) ^ (m.key0 + kPhiloxW0), (unsigned)q, (unsigned)p};
 }
 __device__ __forceinline__ MaskRow mask_row(const Mask& m, int64_t row) {
-  const uint64_t r = (uint64_t)(row + m.row0);
+  const uint64_t r = (uint64_t)row + (uint64_t)m.row0;
   const uint64_t q = (uint64_t)(unsigned)(r >> 32) * kPhiloxM1;
   const uint64_t p = (uint64_t)xor3((unsigned)(q >> 32), (unsigned)r, m.key0) * kPhiloxM0;
   return {(unsigned)q, (unsigned)(p >> 32) ^ (m.key1 + kPhiloxW1), (unsigned)p};

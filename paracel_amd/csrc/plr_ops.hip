@@ -658,25 +658,68 @@ bool fits_launch(int64_t x, int64_t y, int threads) {
   return y == 0 || x <= (int64_t)0xffffffffu / threads / y;
 }
 
-// Workgroups of the tiled kernels; false when a launch cannot hold them.
-bool tile_grid(int64_t n, int64_t chunks, int tc, int sets, unsigned* nbx, unsigned* grid) {
-  const int64_t x = ceil_div(chunks, (int64_t)1 << tc);
-  const int64_t y = ceil_div(n, (int64_t)(16 >> tc) * sets);
-  if (!fits_launch(x, y, kQuantThreads)) return false;
-  *nbx = (unsigned)x;
-  *grid = (unsigned)(x * y);
-  return true;
+// The tiled kernels over n rows of `chunks` chunks: launch(first row, rows, tiles across, grid) for
+// as many rows at a time as a launch holds.
+template <typename F>
+void over_rows(int64_t n, int64_t chunks, int tc, int sets, F launch) {
+  const int64_t tile = (int64_t)(16 >> tc) * sets;
+  const int64_t x = ceil_div(chunks, (int64_t)1 << tc);  // at most 2^23
+  const int64_t most = (int64_t)0xffffffffu / kQuantThreads / x * tile;
+  for (int64_t r0 = 0; r0 < n; r0 += most) {
+    const int64_t rows = std::min(most, n - r0);
+    launch(r0, rows, (unsigned)x, (unsigned)(x * ceil_div(rows, tile)));
+  }
 }
 
 template <typename T>
-void launch_quantize(const QuantArgs& a, bool transpose, bool drop, unsigned grid, hipStream_t st) {
+void launch_quantize(QuantArgs a, bool transpose, bool drop, unsigned grid, hipStream_t st) {
   if (transpose) {
     auto f = drop ? quantize_columns<T, true> : quantize_columns<T, false>;
     hipLaunchKernelGGL(f, dim3(grid), dim3(64 * kColumnWaves), 0, st, a);
   } else {
     auto f = drop ? quantize_rows<T, true> : quantize_rows<T, false>;
-    hipLaunchKernelGGL(f, dim3(grid), dim3(kQuantThreads), 0, st, a);
+    a.tc_log2 = tile_log2(a.chunks);
+    over_rows(a.n, a.chunks, a.tc_log2, kQuantRows<T>, [&](int64_t r0, int64_t rows, unsigned x, unsigned g) {
+      QuantArgs b = a;
+      b.x = static_cast<const T*>(a.x) + r0 * a.ldx;
+      b.codes += r0 * a.ldc;
+      b.scales += r0 * a.lds;
+      b.mask.row0 = (int64_t)((uint64_t)a.mask.row0 + (uint64_t)r0);
+      b.n = rows;
+      b.nbx = x;
+      hipLaunchKernelGGL(f, dim3(g), dim3(kQuantThreads), 0, st, b);
+    });
   }
+}
+
+template <typename T>
+void launch_dequantize(DequantArgs a, hipStream_t st) {
+  const int64_t chunks = ceil_div(a.d, 128);
+  a.tc_log2 = tile_log2(chunks);
+  over_rows(a.n, chunks, a.tc_log2, kMoveRows<T>, [&](int64_t r0, int64_t rows, unsigned x, unsigned g) {
+    DequantArgs b = a;
+    b.codes += r0 * a.ldc;
+    b.scales += r0 * a.lds;
+    b.out = static_cast<T*>(a.out) + r0 * a.ldo;
+    b.n = rows;
+    b.nbx = x;
+    hipLaunchKernelGGL(dequantize_rows<T>, dim3(g), dim3(kQuantThreads), 0, st, b);
+  });
+}
+
+template <typename T>
+void launch_dropout(DropArgs a, hipStream_t st) {
+  const int64_t chunks = ceil_div(a.d, 128);
+  a.tc_log2 = tile_log2(chunks);
+  over_rows(a.n, chunks, a.tc_log2, kMoveRows<T>, [&](int64_t r0, int64_t rows, unsigned x, unsigned g) {
+    DropArgs b = a;
+    b.x = static_cast<const T*>(a.x) + r0 * a.ldx;
+    b.out = static_cast<T*>(a.out) + r0 * a.ldo;
+    b.mask.row0 = (int64_t)((uint64_t)a.mask.row0 + (uint64_t)r0);
+    b.n = rows;
+    b.nbx = x;
+    hipLaunchKernelGGL(dropout_rows<T>, dim3(g), dim3(kQuantThreads), 0, st, b);
+  });
 }
 
 }  // namespace
@@ -733,10 +776,6 @@ int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned 
     if (!fits_launch(x, y, 64 * kColumnWaves)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
     a.nbx = (unsigned)x;
     grid = (unsigned)(x * y);
-  } else {
-    a.tc_log2 = tile_log2(a.chunks);
-    if (!tile_grid(n, a.chunks, a.tc_log2, size == 2 ? kQuantRows<__bf16> : kQuantRows<float>, &a.nbx, &grid))
-      return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   }
   rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || n == 0) return rc;
@@ -778,19 +817,13 @@ int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, 
   a.n = n;
   a.d = d;
   a.ldo = ldo;
-  const int64_t chunks = ceil_div(d, 128);
-  a.tc_log2 = tile_log2(chunks);
-  unsigned grid = 0;
-  if (!tile_grid(n, chunks, a.tc_log2, size == 2 ? kMoveRows<__bf16> : kMoveRows<float>, &a.nbx, &grid))
-    return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   int rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || n == 0) return rc;
-  const dim3 g(grid), t(kQuantThreads);
   switch (type) {
-    case PLR_F64: hipLaunchKernelGGL(dequantize_rows<double>, g, t, 0, c.stream, a); break;
-    case PLR_F32: hipLaunchKernelGGL(dequantize_rows<float>, g, t, 0, c.stream, a); break;
-    case PLR_BF16: hipLaunchKernelGGL(dequantize_rows<__bf16>, g, t, 0, c.stream, a); break;
-    default: hipLaunchKernelGGL(dequantize_rows<_Float16>, g, t, 0, c.stream, a); break;
+    case PLR_F64: launch_dequantize<double>(a, c.stream); break;
+    case PLR_F32: launch_dequantize<float>(a, c.stream); break;
+    case PLR_BF16: launch_dequantize<__bf16>(a, c.stream); break;
+    default: launch_dequantize<_Float16>(a, c.stream); break;
   }
   return c.launched();
 }
@@ -818,19 +851,13 @@ int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned 
   a.d = d;
   a.ldx = ldx;
   a.ldo = ldo;
-  const int64_t chunks = ceil_div(d, 128);
-  a.tc_log2 = tile_log2(chunks);
-  unsigned grid = 0;
-  if (!tile_grid(n, chunks, a.tc_log2, size == 2 ? kMoveRows<__bf16> : kMoveRows<float>, &a.nbx, &grid))
-    return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
   rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || n == 0) return rc;
-  const dim3 g(grid), t(kQuantThreads);
   switch (type) {
-    case PLR_F64: hipLaunchKernelGGL(dropout_rows<double>, g, t, 0, c.stream, a); break;
-    case PLR_F32: hipLaunchKernelGGL(dropout_rows<float>, g, t, 0, c.stream, a); break;
-    case PLR_BF16: hipLaunchKernelGGL(dropout_rows<__bf16>, g, t, 0, c.stream, a); break;
-    default: hipLaunchKernelGGL(dropout_rows<_Float16>, g, t, 0, c.stream, a); break;
+    case PLR_F64: launch_dropout<double>(a, c.stream); break;
+    case PLR_F32: launch_dropout<float>(a, c.stream); break;
+    case PLR_BF16: launch_dropout<__bf16>(a, c.stream); break;
+    default: launch_dropout<_Float16>(a, c.stream); break;
   }
   return c.launched();
 }

@@ -169,6 +169,48 @@ def _keep_columns(n, c0, c1, drop):
     return np.stack(parts, -1).reshape(n, -1)[:, :c1 - c0] >= ref.threshold(drop.rate)
 
 
+def test_more_rows_than_a_launch_holds(capi):
+    # 300 million rows of two values
+    n, d, tail = 300000001, 2, 1000
+    rng = np.random.default_rng(4)
+    x = rng.normal(size=(tail, d)).astype(np.float32)
+    drop = capi.Dropout(0.5, 9, 2, 1 << 33)
+    keep = ref.keep(tail, d, capi.Dropout(0.5, 9, 2, (1 << 33) + n - tail))
+    dx = Big(n * d * 4)
+    dx.put((n - tail) * d * 4, x)
+    codes, scales = Big(n * 16), Big(n)
+    capi.mxfp_quantize(dx.ptr, 1, n, d, d, codes.ptr, 16, scales.ptr, 1, drop=drop)
+    want = np.where(keep, x, 0).astype(np.float64)
+    c, s = ref.quantize(want)
+    assert np.array_equal(codes.get((n - tail) * 16, (tail, 16), np.uint8), ref.pack(c, s, 16, 1)[0])
+    assert np.array_equal(scales.get(n - tail, (tail, 1), np.uint8), s)
+    capi.dropout_apply(dx.ptr, 1, n, d, d, dx.ptr, d, drop)
+    assert np.array_equal(dx.get((n - tail) * d * 4, (tail, d), np.float32), 2 * want.astype(np.float32))
+    capi.mxfp_dequantize(codes.ptr, 16, scales.ptr, 1, n, d, dx.ptr, 1, d)
+    assert np.array_equal(dx.get((n - tail) * d * 4, (tail, d), np.float32), ref.rounded(want))
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_product_of_more_rows_than_the_few_rows_kernel_takes(capi, swap):
+    many, few, k, tail = 140000003, 3, 8, 500
+    rng = np.random.default_rng(5)
+    a, b = ref.quantize(rng.normal(size=(tail, k))), ref.quantize(rng.normal(size=(few, k)))
+    da, ds, out = Big(many * 64), Big(many * 4), Big(many * few * 4)
+    for big, part, size in zip((da, ds), ref.pack(*a, 64, 4), (64, 4)):
+        big.put((many - tail) * size, part)
+    cb, sb = (ref.Dev(t) for t in ref.pack(*b, 64, 4))
+    va, vb = ref.values(*a)[:, :k], ref.values(*b)[:, :k]
+    one, two = (da.ptr, 64, ds.ptr, 4), (cb.ptr, 64, sb.ptr, 4)
+    bound = _bound(va, vb, k, va @ vb.T, 1)
+    if swap:
+        capi.mxfp_matmul(few, many, k, *two, *one, out.ptr, 1, many)
+        got = np.stack([out.get((i * many + many - tail) * 4, (tail,), np.float32) for i in range(few)], 1)
+    else:
+        capi.mxfp_matmul(many, few, k, *one, *two, out.ptr, 1, few)
+        got = out.get((many - tail) * few * 4, (tail, few), np.float32)
+    assert (np.abs(got - va @ vb.T) <= bound).all()
+
+
 def test_shard(plr):
     # 2.2e6 x 4096: 4.8 GB of codes, 72 GB before them; every 20000 rows repeat, so sums are known
     from paracel_amd import Dropout

@@ -173,6 +173,9 @@ def test_empty_shard_and_refusals(plr):
             call()
         assert e.value.code == -5 and "pack" in str(e.value)
     plr.calc_loss(theta)
+    plr.set_dropout(Dropout(0.0, 1))  # drops nothing: none
+    plr.loss_grad(theta)
+    plr.set_dropout(Dropout(0.5, 1))
     plr.pack_data()
     plr.pack_data()  # packed already: nothing to do
     plr.loss_grad(theta)
