@@ -222,6 +222,7 @@ struct PackedFns {
   int sets;           // row sets of a tile
   int threads;
   int most_slots;     // rows side by side
+  bool sums;          // of a gradient
   packed_fn fn;
 };
 enum { kGrad, kGradDrop, kEval };
@@ -230,9 +231,9 @@ struct PackedFused {
 };
 template <int STRIDE, int SR, int NT, int MINW>
 constexpr PackedFused make_packed() {
-  return {{{STRIDE, SR, NT, NT, plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>},
-           {STRIDE, SR, NT, NT, plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
-           {STRIDE, SR, NT, NT, plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>}}};
+  return {{{STRIDE, SR, NT, NT, true, plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>},
+           {STRIDE, SR, NT, NT, true, plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
+           {STRIDE, SR, NT, NT, false, plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>}}};
 }
 // Row sets per tile: as many as leave two workgroups (of 512 threads one) on a compute unit; the
 // barriers and row terms of a tile cost the same however long it is (1M x 1000: 16 sets 265 us,
@@ -250,11 +251,11 @@ struct PackedSweep {
 };
 template <int SR, int NT, int MINW, bool DROP>
 constexpr PackedFns make_dot() {
-  return {kDotPiece, SR, NT, kSweepSlots, plr::packed_pass<false, DROP, plr::kPassDot, kDotPiece, SR, NT, MINW>};
+  return {kDotPiece, SR, NT, kSweepSlots, false, plr::packed_pass<false, DROP, plr::kPassDot, kDotPiece, SR, NT, MINW>};
 }
 template <int SR, int NT, int MINW, bool DROP>
 constexpr PackedFns make_axpy() {
-  return {0, SR, NT, kSweepSlots, plr::packed_pass<true, DROP, plr::kPassAxpy, 0, SR, NT, MINW>};
+  return {0, SR, NT, kSweepSlots, true, plr::packed_pass<true, DROP, plr::kPassAxpy, 0, SR, NT, MINW>};
 }
 const PackedSweep kDot = {kDotPiece, {make_dot<8, 512, 4, false>(), make_dot<8, 512, 2, true>()}};
 const PackedSweep kAxpy = {kAxpyPiece, {make_axpy<8, 768, 3, false>(), make_axpy<8, 512, 2, true>()}};
@@ -639,15 +640,16 @@ int packed_slots(const PackedFns* f, int64_t blocks) {
 }
 
 // LDS: theta, partial dot products, residuals and (with dropout, between the halves of a fused
-// pass) marks of a tile, and in the end 9 doubles a thread; of a row's widest and narrowest piece.
+// pass) marks of a tile, of a row's widest and narrowest piece; in the end the gradient sums.
 size_t packed_lds(const PackedFns* f, int64_t row_blocks, int64_t piece, bool marks) {
   auto one = [&](int64_t blocks) {
     const size_t rows = f->stride ? (size_t)packed_slots(f, blocks) * f->sets : 0;
-    return std::max((size_t)f->threads * 9, (size_t)32 * f->stride + rows * ((blocks | 1) + 1)) * sizeof(double) +
+    return ((size_t)32 * f->stride + rows * ((blocks | 1) + 1)) * sizeof(double) +
            (marks ? (size_t)f->sets * f->threads * sizeof(unsigned) : 0);
   };
+  const size_t end = f->sums ? (size_t)f->threads * (plr::packed_end_columns(f->threads) + 1) * sizeof(double) : 0;
   const int64_t over = row_blocks % piece;
-  return std::max(one(std::min(piece, row_blocks)), over ? one(over) : 0);
+  return std::max({end, one(std::min(piece, row_blocks)), over ? one(over) : 0});
 }
 
 const PackedFused& packed_fused_for(int64_t blocks) {

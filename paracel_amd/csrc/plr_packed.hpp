@@ -99,6 +99,8 @@ __device__ __forceinline__ double tile_scale(const PackedTile<R>& t, int r) {
 }
 
 constexpr int kPackedR = 4;
+// Columns of a block whose sums meet in LDS at a time: all, where a workgroup's fit.
+constexpr int packed_end_columns(int threads) { return threads <= 512 ? 32 : 8; }
 
 // The marks (bit q + 4 i: column 8 q + i) of a block's columns from `left` on.
 __device__ __forceinline__ unsigned columns_behind(int64_t left) {
@@ -319,28 +321,29 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
     }
   }
   if (GRAD) {
-    // The slots' sums, eight columns at a time: `share8` threads to a column, each in slot order,
-    // then among themselves.  (9 doubles per thread keep a column's slots on different banks.)
-    int share8 = 1;
-    while (share8 < kWave && share8 * 2 * blocks * 8 <= NT && share8 < slots) share8 *= 2;
-    __syncthreads();
+    // The slots' sums, EC columns of a block at a time: `share` threads to a column, each in slot
+    // order, then among themselves.  (EC + 1 doubles per thread keep a column's slots on different
+    // banks.)
+    constexpr int EC = packed_end_columns(NT);
+    int share = 1;
+    while (share < kWave && share * 2 * blocks * EC <= NT && share < slots) share *= 2;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int c0 = 0; c0 < 32; c0 += EC) {
+      __syncthreads();
       if (active) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sm[tid * 9 + i] = acc[8 * q + i];
+        for (int i = 0; i < EC; ++i) sm[tid * (EC + 1) + i] = acc[c0 + i];
       }
       __syncthreads();
-      for (int e0 = 0; e0 < blocks * 8; e0 += NT / share8) {
-        const int e = e0 + tid / share8, b = e >> 3, i = e & 7;
+      for (int e0 = 0; e0 < blocks * EC; e0 += NT / share) {
+        const int e = e0 + tid / share, b = e / EC, i = e % EC;
         double g = 0.;
         if (b < blocks)
-          for (int s = tid & (share8 - 1); s < slots; s += share8) g += sm[(s * blocks + b) * 9 + i];
-        for (int m = 1; m < share8; m <<= 1) g += __shfl_xor(g, m, kWave);
-        if (b < blocks && (tid & (share8 - 1)) == 0)
-          a.part_g[(int64_t)blockIdx.x * a.pitch + (int64_t)(blk0 + b) * 32 + 8 * q + i] = g;
+          for (int s = tid & (share - 1); s < slots; s += share) g += sm[(s * blocks + b) * (EC + 1) + i];
+        for (int m = 1; m < share; m <<= 1) g += __shfl_xor(g, m, kWave);
+        if (b < blocks && (tid & (share - 1)) == 0)
+          a.part_g[(int64_t)blockIdx.x * a.pitch + (int64_t)(blk0 + b) * 32 + c0 + i] = g;
       }
-      __syncthreads();
     }
   }
   if (MODE == kPassFused) emit_row_sums<NT / kWave>(sums, lane, wave, a.part_loss, a.part_res);
