@@ -213,9 +213,8 @@ int g_na_num_cu[kNaMaxDevices] = {};
 int g_na_occ[kNaMaxDevices][kNaMaxPitch / plr::kChunkCols + 1] = {};
 std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 
-// Shard held in 4 bits.  A row of up to kPackedFused blocks is read once (theta and the partial
-// dot products of two tiles have to fit a compute unit's LDS); wider ones go in column pieces, in
-// two sweeps.
+// Shard held in 4 bits.  Narrow rows are read once, theta and a tile's partial dot products in LDS;
+// wide ones go in column pieces, in two sweeps, where no wave waits for a whole row.
 typedef void (*packed_fn)(plr::PackedArgs);
 struct PackedFns {
   int stride;         // blocks of theta in LDS (none: 0): the widest row or piece
@@ -229,22 +228,27 @@ enum { kGrad, kGradDrop, kEval };
 struct PackedFused {
   PackedFns fns[3];
 };
-template <int STRIDE, int SR, int NT, int MINW>
+template <int STRIDE, int SR, int NT, int MINW, bool EVAL>
 constexpr PackedFused make_packed() {
   return {{{STRIDE, SR, NT, NT, true, plr::packed_pass<true, false, plr::kPassFused, STRIDE, SR, NT, MINW>},
            {STRIDE, SR, NT, NT, true, plr::packed_pass<true, true, plr::kPassFused, STRIDE, SR, NT, MINW>},
-           {STRIDE, SR, NT, NT, false, plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW>}}};
+           {STRIDE, SR, NT, NT, false, EVAL ? plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW> : nullptr}}};
 }
 // Row sets per tile: as many as leave two workgroups (of 512 threads one) on a compute unit; the
 // barriers and row terms of a tile cost the same however long it is (1M x 1000: 16 sets 265 us,
 // 8 sets 301).  Rows of up to 8 blocks lie 32 and more side by side: with 8 sets their partials
 // stay small enough (1M x 100 with dropout: 8 sets 80 us, 16 sets 92).
-const PackedFused kPacked[4] = {make_packed<8, 8, 256, 2>(), make_packed<64, 16, 256, 2>(),
-                              make_packed<256, 8, 512, 2>(), make_packed<512, 4, 512, 2>()};
+const PackedFused kPacked[3] = {make_packed<8, 8, 256, 2, true>(), make_packed<64, 16, 256, 2, true>(),
+                              make_packed<256, 8, 512, 2, false>()};
+// Most blocks of a row that is read once, for a gradient, one with dropout (two sweeps make every
+// mask twice) and no gradient.  Once / two sweeps: 40000 x 4100 78 / 66 us, 123 / 141, 48 / 34;
+// 60000 x 3000 70 / 69, 111 / 151, 44 / 35; 200000 x 1000 65 / 73, 107 / 163, 36 / 37; 60000 x 9000
+// 297 / 159, 505 / 391, 195 / 79.
+constexpr int kPackedFused[3] = {128, 256, 64};
 // The sweeps wait for memory more than they compute: as many waves as their registers allow, in the
 // second one side by side in one workgroup, whose sums then leave it as one (12000 x 16385: three
 // workgroups of 256 threads 81 us a pass, one of 768 79; 3000 x 40001: 72 and 57).
-constexpr int kPackedFused = 480, kDotPiece = 128, kAxpyPiece = 256, kSweepSlots = 64;
+constexpr int kDotPiece = 128, kAxpyPiece = 256, kSweepSlots = 64;
 struct PackedSweep {
   int most_blocks;  // of a piece
   PackedFns fns[2];  // [dropout]
@@ -258,7 +262,7 @@ constexpr PackedFns make_axpy() {
   return {0, SR, NT, kSweepSlots, true, plr::packed_pass<true, DROP, plr::kPassAxpy, 0, SR, NT, MINW>};
 }
 const PackedSweep kDot = {kDotPiece, {make_dot<8, 512, 4, false>(), make_dot<8, 512, 2, true>()}};
-const PackedSweep kAxpy = {kAxpyPiece, {make_axpy<8, 768, 3, false>(), make_axpy<8, 512, 2, true>()}};
+const PackedSweep kAxpy = {kAxpyPiece, {make_axpy<8, 768, 3, false>(), make_axpy<8, 768, 3, true>()}};
 
 }  // namespace
 
@@ -276,6 +280,11 @@ struct PackedLaunch {
   int64_t piece = 0, steps = 0;  // blocks; groups of row sets per workgroup
   int pieces = 0, grid = 0;
   size_t lds = 0;
+};
+
+struct PackedPlan {
+  bool sweeps = false;     // column pieces, two sweeps
+  PackedLaunch pass, dot;  // the only or second sweep, the first one
 };
 
 struct plr_ctx {
@@ -372,9 +381,9 @@ struct plr_ctx {
   uint8_t* d_codes = nullptr;     // n x row_blocks * 16 bytes
   uint8_t* d_scales = nullptr;    // n x row_blocks
   int64_t row_blocks = 0;
-  PackedLaunch packed_plan[3];    // a gradient, one with dropout, none
-  PackedLaunch packed_dot[2];     // two sweeps: the first
-  bool packed_sweeps = false;     // too wide for one read: column pieces, two sweeps
+  unsigned* d_marks = nullptr;    // dropout in two sweeps, allocated by the first such pass
+  PackedPlan packed_plan[3];      // a gradient, one with dropout, none
+  bool packed_sweeps = false;     // one of them in two sweeps
   bool drop_on = false;           // plr_set_dropout
   plr_dropout drop = {0., 0, 0, 0};
 
@@ -416,6 +425,8 @@ void free_shape(plr_ctx* c) {
   release_upload_staging(c);
   if (c->dX) (void)hipFree(c->dX);
   if (c->d_codes) (void)hipFree(c->d_codes);
+  if (c->d_marks) (void)hipFree(c->d_marks);
+  c->d_marks = nullptr;
   if (c->d_scales) (void)hipFree(c->d_scales);
   c->d_codes = c->d_scales = nullptr;
   c->packed = c->packed_sweeps = false;
@@ -653,13 +664,16 @@ size_t packed_lds(const PackedFns* f, int64_t row_blocks, int64_t piece, bool ma
 }
 
 const PackedFused& packed_fused_for(int64_t blocks) {
-  return kPacked[blocks <= 8 ? 0 : blocks <= 64 ? 1 : blocks <= 256 ? 2 : 3];
+  return kPacked[blocks <= 8 ? 0 : blocks <= 64 ? 1 : 2];
 }
 
 // Rows the kernels may read behind the last one: less than a group of row sets of any launch.
 int64_t packed_slack_rows(int64_t row_blocks) {
-  return (int64_t)plr::kPackedR * (row_blocks > kPackedFused ? kSweepSlots
-                                                             : packed_slots(&packed_fused_for(row_blocks).fns[kGrad], row_blocks));
+  int64_t slots = 0;
+  for (int k = kGrad; k <= kEval; ++k)
+    slots = std::max<int64_t>(slots, row_blocks > kPackedFused[k]
+                                         ? kSweepSlots : packed_slots(&packed_fused_for(row_blocks).fns[k], row_blocks));
+  return slots * plr::kPackedR;
 }
 
 // One launch over n rows: its kernel, the blocks of a column piece and its persistent grid.
@@ -696,30 +710,32 @@ int plan_packed_sweep(plr_ctx* c, const PackedSweep& s, bool drop, int64_t n, Pa
 int plan_packed(plr_ctx* c, int64_t n) {
   c->row_blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
   c->pitch = c->theta_len = c->row_blocks * plr_mx::kBlockCols;
-  c->packed_sweeps = c->row_blocks > kPackedFused;
+  c->packed_sweeps = false;
   c->var = &kBlockShape;  // unused by this path, kept non-null
   c->nch_rt = 1;
-  int rc = PLR_OK;
-  if (c->packed_sweeps) {
-    for (int k = 0; k < 2 && rc == PLR_OK; ++k) {
-      rc = plan_packed_sweep(c, kAxpy, k == 1, n, &c->packed_plan[k]);
-      if (rc == PLR_OK) rc = plan_packed_sweep(c, kDot, k == 1, n, &c->packed_dot[k]);
+  for (int k = kGrad; k <= kEval; ++k) {
+    PackedPlan& p = c->packed_plan[k];
+    p.sweeps = c->row_blocks > kPackedFused[k];
+    int rc = PLR_OK;
+    if (p.sweeps) {
+      c->packed_sweeps = true;
+      rc = plan_packed_sweep(c, kDot, k == kGradDrop, n, &p.dot);
+      if (k == kEval) p.pass = p.dot;
+      else if (rc == PLR_OK) rc = plan_packed_sweep(c, kAxpy, k == kGradDrop, n, &p.pass);
+    } else {
+      rc = plan_packed_launch(c, &packed_fused_for(c->row_blocks).fns[k], n, c->row_blocks, k == kGradDrop, &p.pass);
     }
-    c->packed_plan[kEval] = c->packed_dot[0];
-  } else {
-    const PackedFused& f = packed_fused_for(c->row_blocks);
-    for (int k = kGrad; k <= kEval && rc == PLR_OK; ++k)
-      rc = plan_packed_launch(c, &f.fns[k], n, c->row_blocks, k == kGradDrop, &c->packed_plan[k]);
+    if (rc != PLR_OK) return rc;
   }
-  if (rc != PLR_OK) return rc;
-  const PackedLaunch &lg = c->packed_plan[kGrad], &ld = c->packed_plan[kGradDrop], &le = c->packed_plan[kEval];
+  const PackedLaunch &lg = c->packed_plan[kGrad].pass, &ld = c->packed_plan[kGradDrop].pass,
+                     &le = c->packed_plan[kEval].pass;
   c->grid = std::max(lg.grid, ld.grid);
   c->grid_nograd = le.grid;
   char b[256];
   snprintf(b, sizeof b,
            "packed_pass<SR=%d> 4-bit shard, %lld blocks of 32 columns per row%s, %d rows side by side, "
            "grid=%d x %d threads (%d with dropout, %d without a gradient)",
-           lg.fns->sets, (long long)c->row_blocks, c->packed_sweeps ? " in pieces, two sweeps" : "",
+           lg.fns->sets, (long long)c->row_blocks, c->packed_plan[kGrad].sweeps ? " in pieces, two sweeps" : "",
            packed_slots(lg.fns, lg.piece), lg.grid * lg.pieces, lg.fns->threads, ld.grid * ld.pieces,
            le.grid * le.pieces);
   c->info = b;
@@ -801,7 +817,9 @@ int alloc_workspace(plr_ctx* c) {
     PLR_HIP(c, hipMalloc(&c->d_zparts, (size_t)c->zstride * c->nteams * c->team_blocks *
                                            plr::kTeamWaves * sizeof(double)));
   } else if ((c->blocked || c->packed_sweeps) && n > 0) {
-    const int64_t parts = c->packed_sweeps ? std::max(c->packed_dot[0].pieces, c->packed_dot[1].pieces) : 1;
+    int64_t parts = 1;  // of a row's dot product
+    for (const PackedPlan& p : c->packed_plan)
+      if (c->packed_sweeps && p.sweeps) parts = std::max<int64_t>(parts, p.dot.pieces);
     PLR_HIP(c, hipMalloc(&c->d_z, (size_t)n * parts * sizeof(double)));
     PLR_HIP(c, hipMalloc(&c->d_res, (size_t)n * sizeof(double)));
   }
@@ -874,6 +892,7 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
   a.part_res = pa.part_res;
   a.h_out = pa.h_out;
   a.z_buf = c->d_z;
+  a.marks = c->d_marks;
   a.res_in = c->d_res;
   a.n = c->n;
   a.row_blocks = c->row_blocks;
@@ -896,19 +915,19 @@ int enqueue_packed(plr_ctx* c, const PassArgs& pa, bool grad, int train_round, i
     hipLaunchKernelGGL(l.fns->fn, dim3(l.grid, l.pieces), dim3(l.fns->threads), l.lds, c->stream, a);
     return hipGetLastError();
   };
-  const PackedLaunch& plan = c->packed_plan[!grad ? kEval : drop ? kGradDrop : kGrad];
-  *parts = *loss_parts = plan.grid;
-  if (!c->packed_sweeps) {
-    PLR_HIP(c, launch(plan));
+  const PackedPlan& plan = c->packed_plan[!grad ? kEval : drop ? kGradDrop : kGrad];
+  *parts = *loss_parts = plan.pass.grid;
+  if (!plan.sweeps) {
+    PLR_HIP(c, launch(plan.pass));
     return PLR_OK;
   }
-  PLR_HIP(c, launch(c->packed_dot[drop]));
+  PLR_HIP(c, launch(plan.dot));
   hipLaunchKernelGGL(plr::packed_residual, dim3(c->res_grid), dim3(256), 0, c->stream, (const double*)c->d_z,
-                     c->packed_dot[drop].pieces, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
+                     plan.dot.pieces, (const double*)pa.y, grad ? c->d_res : nullptr, pa.h_out,
                      c->d_part_loss, c->n, pa.loss_mode, pa.identity_link, pa.theta_bias, pa.part_res);
   PLR_HIP(c, hipGetLastError());
   *loss_parts = c->res_grid;
-  if (grad) PLR_HIP(c, launch(plan));
+  if (grad) PLR_HIP(c, launch(plan.pass));
   return PLR_OK;
 }
 
@@ -1215,11 +1234,17 @@ bool results_arrived(plr_ctx* c) {
   }
 }
 
-// Dropout belongs to the passes over a shard held in 4 bits.
+// Dropout belongs to the passes over a shard held in 4 bits; in two sweeps the second reads what the
+// first dropped (a bit per value: the generator again costs three times the bytes it saves).
 int check_dropout(plr_ctx* c) {
   if (c->drop_on && !c->packed)
     return fail(c, PLR_ERR_UNSUPPORTED,
                 "dropout is set, but the resident shard is one of doubles: call plr_pack_data first");
+  if (c->drop_on && c->packed_plan[kGradDrop].sweeps && !c->d_marks && c->n > 0) {
+    PLR_HIP(c, hipSetDevice(c->device));
+    PLR_HIP(c, hipMalloc(&c->d_marks, ((size_t)c->n + packed_slack_rows(c->row_blocks)) * c->row_blocks *
+                                          sizeof(unsigned)));
+  }
   return PLR_OK;
 }
 

@@ -38,6 +38,7 @@ struct PackedArgs {
   double* part_res;       // [grid] or nullptr
   double* h_out;          // n or nullptr
   double* z_buf;          // kPassDot: [pieces][n], each piece's part of the dot products
+  unsigned* marks;        // two sweeps with dropout: what the first one dropped, a word per block
   const double* res_in;   // kPassAxpy: n
   int64_t n;
   int64_t row_blocks;     // blocks of a stored row
@@ -64,7 +65,8 @@ template <int R>
 struct PackedLoads {
   uint4 codes[R];
   unsigned char scales[R];
-  double res[R];  // kPassAxpy
+  double res[R];      // kPassAxpy
+  unsigned marks[R];  // kPassAxpy with dropout
 };
 template <int R>
 __device__ __forceinline__ PackedTile<R> arrived(const PackedLoads<R>& l) {
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) acc[i] = 0.;
   plr_mx::MaskGroup group[4];
-  if (DROP) {
+  if (DROP && MODE != kPassAxpy) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) group[q] = plr_mx::mask_group(a.mask, (unsigned)((blk0 + blk) * 4 + q));
   }
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
       const int64_t at = (set + r) * slots * a.row_blocks;  // the same for all threads
       t.codes[r] = reinterpret_cast<const uint4*>(a.codes + at * 16)[at_lane];
       t.scales[r] = (a.scales + at)[at_lane];
+      if (MODE == kPassAxpy && DROP) t.marks[r] = (a.marks + at)[at_lane];
       if (MODE == kPassAxpy) t.res[r] = a.res_in[min((set + r) * slots + slot, a.n - 1)];
     }
   };
@@ -228,6 +231,10 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
 #pragma unroll
             for (int r = 0; r < R; ++r) ml[(s + r) * NT + tid] = marks[r];
           }
+          if (MODE == kPassDot && active) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) (a.marks + (set0 + s + r) * slots * a.row_blocks)[at_lane] = marks[r];
+          }
         }
         double part[R][2];
 #pragma unroll
@@ -292,15 +299,14 @@ __global__ __launch_bounds__(NT, MINW) void packed_pass(PackedArgs a) {
         double w[R];
         if (MODE == kPassAxpy) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) w[r] = nxt.res[r];
+          for (int r = 0; r < R; ++r) {
+            w[r] = nxt.res[r];
+            if (DROP) drop_again(cur, r, nxt.marks[r]);
+          }
         }
         if (s + R < sets) load(set0 + s + R, nxt);
         else if (more) load(set0 + SR, nxt);
         if (MODE == kPassAxpy) {
-          if (DROP) {
-            unsigned marks[R];
-            drop(set0 + s, cur, marks);
-          }
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const int64_t row = (set0 + s + r) * slots + slot;

@@ -12,7 +12,7 @@ REL = 1e-11
 
 SHAPES = [(1, 1), (5, 2), (1000, 31), (777, 32), (64, 33), (5000, 41), (3000, 100), (1234, 257),
           (2500, 512), (1001, 1000), (999, 1100), (300, 2049), (257, 2080), (130, 4100), (67, 8193),
-          (40, 16384), (33, 16385), (21, 20000), (3, 40001), (1, 1000), (20000, 3), (700, 15361), (200, 30000)]
+          (40, 16384), (90, 2080), (60, 4097), (70, 8160), (50, 8193), (33, 16385), (21, 20000), (3, 40001), (1, 1000), (20000, 3), (700, 15361), (200, 30000)]
 
 
 def close(got, want, rel=REL):
