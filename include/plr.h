@@ -301,7 +301,9 @@ int plr_pack_data(plr_ctx* ctx);
  * as given, so a caller names a new one every round.  The loss of such a pass
  * is that of the dropped values; plr_calc_loss and plr_predict never drop.
  * On a shard of doubles these passes fail with PLR_ERR_UNSUPPORTED while
- * dropout is set (plr_dropout_apply and plr_loss_grad_noalloc serve there). */
+ * dropout is set (plr_dropout_apply and plr_loss_grad_noalloc serve there).
+ * Rows of more than 8192 columns take scratch memory of a bit per value, which
+ * the first such pass allocates. */
 int plr_set_dropout(plr_ctx* ctx, const plr_dropout* drop);
 
 /* Block until everything this context (and the device) was asked to do has

@@ -240,10 +240,10 @@ constexpr PackedFused make_packed() {
 // stay small enough (1M x 100 with dropout: 8 sets 80 us, 16 sets 92).
 const PackedFused kPacked[3] = {make_packed<8, 8, 256, 2, true>(), make_packed<64, 16, 256, 2, true>(),
                               make_packed<256, 8, 512, 2, false>()};
-// Most blocks of a row that is read once, for a gradient, one with dropout (two sweeps make every
-// mask twice) and no gradient.  Once / two sweeps: 40000 x 4100 78 / 66 us, 123 / 141, 48 / 34;
-// 60000 x 3000 70 / 69, 111 / 151, 44 / 35; 200000 x 1000 65 / 73, 107 / 163, 36 / 37; 60000 x 9000
-// 297 / 159, 505 / 391, 195 / 79.
+// Most blocks of a row that is read once, for a gradient, one with dropout and no gradient.  Once and
+// in two sweeps, us: 200000 x 1000 65 and 73, 107 and 163, 36 and 37; 60000 x 3000 70 and 69, 109 and
+// 121, 44 and 35; 40000 x 4100 78 and 66, 123 and 121, 48 and 34; 30000 x 8000 90 and 85, 138 and 152,
+// 54 and 44; 60000 x 9000 297 and 159, 505 and 325, 195 and 79.
 constexpr int kPackedFused[3] = {128, 256, 64};
 // The sweeps wait for memory more than they compute: as many waves as their registers allow, in the
 // second one side by side in one workgroup, whose sums then leave it as one (12000 x 16385: three

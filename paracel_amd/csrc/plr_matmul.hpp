@@ -136,7 +136,7 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned 
 // waits are the step's own.
 __device__ __forceinline__ void copy_to_lds(const uint8_t* base, unsigned offset, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               ::"s"(lds), "v"(offset), "s"(base) : "memory");
+               ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -144,7 +144,7 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 
 __device__ __forceinline__ void copy_word_to_lds(const uint8_t* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-               ::"s"(lds), "v"(src) : "memory");
+               ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
 template <typename T, bool DROP, int BM, int BN, int WM, int WN>
