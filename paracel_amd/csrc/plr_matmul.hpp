@@ -128,6 +128,9 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned 
 // 64 bytes of a stage the four blocks are permuted by the row number, so that the 16 rows a wave
 // reads at once lie on different banks.
 //
+// 8192^3 in 280 us, 3.9 PFLOP/s; bound by power (the clock falls to 1.6 GHz) and by LDS: a step takes
+// 1500 cycles, the matrix instructions of its two waves per SIMD 1024.
+//
 // Scales go the same way, 16 bytes per row and group of four steps, in a ring of three groups; a
 // lane picks its block's four bytes into one word once per group, and the instruction selects the
 // byte of its step.
@@ -311,9 +314,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
 
 // ------------------------------------------------------------------- few rows on one side
 // A few rows of the one operand ("few") against many of the other: bound by the bytes of the many,
-// which are read once, straight into the instruction's operands.  A workgroup owns 16 FX rows of
-// the many and 16 FY of the few; its W waves divide k, and their sums meet in LDS in wave order.
-// Codes of four chunks are requested at once: 256 consecutive bytes of a row.  The same, in
+// which are read once, straight into the instruction's operands (1 x 16384 x 8192: 14 us,
+// 5.1 TB/s).  A workgroup owns 16 FX rows of the many and 16 FY of the few; its W waves divide k, and
+// their sums meet in LDS in wave order.  Codes of four chunks are requested at once: 256 consecutive bytes of a row.  The same, in
 // pieces of 64 x 32 and 32 x 32, serves small products, which have too few large tiles to fill the
 // device.  Rows a power of two of bytes apart meet in the same channels of the L2 cache
 // (256 x 256 x 16384: 17 us, where its bytes alone are 4): 16 waves to a piece make it slower.
@@ -422,12 +425,14 @@ __global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
       const int64_t xr = x0 + 16 * x + 4 * q, yr = y0 + 16 * y + r16;
       if (xr >= a.rows || yr >= a.few) continue;
       unsigned drops = 0;
-      if (DROP && !SWAP) drops = drop_marks(a.p.mask, yr + a.p.row0, (unsigned)((xr + a.p.col0) >> 3)) >> 4 * (xr & 7);
+      if (DROP && !SWAP)
+        drops = drop_marks(a.p.mask, yr + a.p.row0, (unsigned)((xr + a.p.col0) >> 3)) >> 4 * (xr & 7);
       T out[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v = a.p.alpha * acc[x][y][e];
-        if (DROP && SWAP) drops = drop_marks(a.p.mask, xr + e + a.p.row0, (unsigned)((yr + a.p.col0) >> 3)) >> 4 * (yr & 7) << 4 * e;
+        if (DROP && SWAP)
+          drops = drop_marks(a.p.mask, xr + e + a.p.row0, (unsigned)((yr + a.p.col0) >> 3)) >> 4 * (yr & 7) << 4 * e;
         if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * a.p.kept;
         out[e] = (T)v;
       }
@@ -456,8 +461,8 @@ inline bool launch_tiles(const MatmulArgs& a, int type, bool drop, hipStream_t s
 template <typename T, bool DROP, int FY, int FX, int W>
 inline void launch_few_as(const FewArgs& a, bool swap, hipStream_t st) {
   auto f = swap ? matmul_few<T, DROP, FY, FX, W, true> : matmul_few<T, DROP, FY, FX, W, false>;
-  hipLaunchKernelGGL(f, dim3((unsigned)((a.rows + 16 * FX - 1) / (16 * FX)), (unsigned)((a.few + 16 * FY - 1) / (16 * FY))),
-                     dim3(64 * W), 0, st, a);
+  const dim3 grid((unsigned)((a.rows + 16 * FX - 1) / (16 * FX)), (unsigned)((a.few + 16 * FY - 1) / (16 * FY)));
+  hipLaunchKernelGGL(f, grid, dim3(64 * W), 0, st, a);
 }
 template <typename T, bool DROP>
 inline void launch_few(const FewArgs& a, bool swap, int cus, int squares, hipStream_t st) {
@@ -504,9 +509,10 @@ inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, i
   a.rows = swap ? p.m : p.n;
   a.few = swap ? p.n : p.m;
   if (a.rows > kMostFewRows || a.few > 65535 * 16) return false;
-  if (type == 0) drop ? launch_few<float, true>(a, swap, cus, squares, st) : launch_few<float, false>(a, swap, cus, squares, st);
-  else if (type == 1) drop ? launch_few<__bf16, true>(a, swap, cus, squares, st) : launch_few<__bf16, false>(a, swap, cus, squares, st);
-  else drop ? launch_few<_Float16, true>(a, swap, cus, squares, st) : launch_few<_Float16, false>(a, swap, cus, squares, st);
+  auto f = type == 0 ? (drop ? launch_few<float, true> : launch_few<float, false>)
+           : type == 1 ? (drop ? launch_few<__bf16, true> : launch_few<__bf16, false>)
+                       : (drop ? launch_few<_Float16, true> : launch_few<_Float16, false>);
+  f(a, swap, cus, squares, st);
   return true;
 }
 
@@ -548,7 +554,8 @@ inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hip
   // A few rows or columns over a multiple of 256 can cost a round of tiles of their own: they go to
   // the kernel for few rows, in a launch of theirs (4096 x 4100 x 2048: 39 us whole, 33 cut).
   const int64_t over_m = a.m % 256 <= 64 ? a.m % 256 : 0, over_n = a.n % 256 <= 64 ? a.n % 256 : 0;
-  if (whole.cut <= kTiles128 && (over_m || over_n) && a.m > 256 && a.n > 256 && std::max(a.m, a.n) <= kMostFewRows) {
+  if (whole.cut <= kTiles128 && (over_m || over_n) && a.m > 256 && a.n > 256 &&
+      std::max(a.m, a.n) <= kMostFewRows) {
     const double cost = plan_matmul(a.m - over_m, a.n - over_n, a.chunks, cus).us +
                         (over_m ? 7 : 0) + (over_n ? 7 : 0);
     if (cost < whole.us) {

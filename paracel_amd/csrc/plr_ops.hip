@@ -275,7 +275,9 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
 }
 
 // Blocks along a row.  A thread takes 8 columns, a quad a block, 16 lanes a chunk of 128 columns;
-// the workgroup's 16 chunk slots are 2^tc across and 16 / 2^tc rows.  Bound by the bytes of x.
+// the workgroup's 16 chunk slots are 2^tc across and 16 / 2^tc rows.  Bound by the bytes of x:
+// 250000 x 512 doubles 190 us, 5.7 TB/s; 16385 x 4100 bfloat16 28 us, 6.2 TB/s, with dropout 44 (there
+// by the generator's 60 instructions per 8 values).
 template <typename T, bool DROP>
 __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
   typedef typename Elem<T>::wide W;
@@ -361,7 +363,8 @@ __device__ __forceinline__ void put_column_block(const QuantArgs& a, const Pack<
 // columns times 32 rows in registers -- so a block never leaves its thread --, 8 lanes cover 128
 // bytes of a row of x and the 8 groups of lanes 256 rows, so that a result row is written in
 // pieces of 128 bytes.  The columns behind the last whole V are left to a wave of their own (the
-// last of a tile row), where a thread takes one column.
+// last of a tile row), where a thread takes one column.  250000 x 512 doubles 211 us, 5.2 TB/s;
+// 16385 x 4100 bfloat16 38 us, with dropout 40: two waves to a SIMD, their tiles fill the registers.
 template <typename T, bool DROP>
 __global__ __launch_bounds__(64 * kColumnWaves, 2) void quantize_columns(QuantArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -473,6 +476,8 @@ struct DequantArgs {
   unsigned nbx;
 };
 
+// The same layout the other way: a lane loads the codes of 8 columns, the quad deals them out.  Bound
+// by the bytes written: 250000 x 512 floats 120 us, 4.8 TB/s (a fill alone 6.9, a copy 5.1).
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) {
   typedef typename Elem<T>::wide W;
@@ -520,7 +525,8 @@ struct DropArgs {
   Mask mask;
 };
 
-// A thread takes 8 columns, one generator call; bound by the bytes moved.
+// A thread takes 8 values, one generator call; bound by the bytes moved: 32768 x 8192 bfloat16 182 us,
+// 5.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void dropout_rows(DropArgs a) {
   typedef typename Elem<T>::wide W;

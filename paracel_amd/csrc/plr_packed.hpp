@@ -3,7 +3,8 @@
 // per value instead of 8, optionally with dropout of the values, arithmetic in 64 bits.
 //
 // Bound by instructions, not bytes: a value costs two multiply-adds in 64 bits and 1.5
-// conversions for each of them, with dropout also an eighth of a generator call.
+// conversions for each of them, with dropout also an eighth of a generator call.  200000 x 1000: 65 us,
+// of which the 6.9 instructions a value that are issued take 39; with dropout 106 and 80 (14.4).
 //
 // A thread owns one block of 32 columns: its gradient sums stay in registers for the kernel's
 // lifetime, theta is in LDS, a row's 32 values are 16 bytes.  A workgroup lays G = threads /
@@ -17,6 +18,9 @@
 // Two barriers per tile.  The row terms are a chain of some 250 dependent instructions; with
 // short tiles (the codes kept in registers from 1 to 3) the workgroup spent half its time there.
 // No atomics: results are reproducible bit for bit.
+//
+// Wide rows go in column pieces and two launches: 1 (kPassDot), packed_residual for 2, 3
+// (kPassAxpy).  12000 x 16385: 35 + 5 + 38 us.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -75,7 +75,7 @@ def test_pitches(capi):
     (dict(lds=3), "scale pitch"), (dict(dx=None), "NULL"), (dict(dcodes=None), "NULL"),
     (dict(dscales=None), "NULL"), (dict(dx=P + 2), "aligned"), (dict(dcodes=P + 8), "aligned"),
     (dict(n=1 << 60), "too large"), (dict(d=1 << 35, ldx=1 << 35), "2^34"),
-    (dict(n=1 << 34, ldc=64, ldx=128, d=100), "one launch"),
+    (dict(n=1 << 34, transpose=True, ldc=1 << 33, lds=1 << 29), "one launch"),
     (dict(device=-1), "device_id"), (dict(device=1000), "device_id"),
 ])
 def test_quantize_refusals(capi, change, what):
