@@ -241,6 +241,7 @@ int64_t plr_mxfp_scale_pitch(int64_t d);
  * behind it are left as they were.
  *   PLR_MXFP_TRANSPOSE  quantises the transpose: d rows of n columns, blocks
  *        along the columns of x -- the operand a gradient's product needs.
+ *        x must fit one launch: 2^32 tiles of 32 rows by 16 bytes.
  *   drop (nullable)  values the mask drops count as 0; kept ones are NOT
  *        multiplied (a power of two is no home for 65536 / (65536 - t): pass
  *        it as alpha to the product).  Rows and columns are those of x, in
