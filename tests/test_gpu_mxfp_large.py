@@ -251,3 +251,32 @@ def test_shard(plr):
     g, l, _ = plr.loss_grad(theta)
     same(g, grad)
     same(np.array([l]), np.array([loss]))
+
+
+@pytest.mark.parametrize("n, d", [(40000003, 2), (9000001, 40), (3000001, 70)])
+def test_narrow_shards(plr, n, d):
+    # rows of the narrow layouts are packed in pieces of 256 MB; a pattern of 1000 rows repeats
+    rng = np.random.default_rng(d)
+    P, theta = rng.normal(size=(1000, d)), rng.normal(size=d)
+    y = (rng.random(1000) < 0.5) * 1.0
+    plr.alloc_data(n, d)
+    step = 3000000
+    for r in range(0, n, step):  # (a multiple of the pattern)
+        m = min(step, n - r)
+        plr.set_data_chunk(r, np.resize(P, (m, d)), np.resize(y, m))
+    plr.pack_data()
+    Q = ref.rounded(P)
+    for at in (0, 16777000, 16777216, 8388000, n - 1000, 838860):
+        if at + 1000 <= n:
+            assert np.array_equal(plr.get_data(at, 1000)[0], np.roll(Q, -(at % 1000), axis=0))
+    times = np.bincount(np.arange(1000), minlength=1000) * (n // 1000) + (np.arange(1000) < n % 1000)
+    z = Q @ theta
+    h = 1 / (1 + np.exp(-z))
+    want = ((h - y) * times) @ Q
+    loss = -(np.where(y == 1, np.log(h), np.log(1 - h)) * times).sum()
+    g, l, rows = plr.loss_grad(theta)
+    assert rows == n and abs(l - loss) <= 1e-10 * abs(loss)
+    # the terms of a column's sum change sign: off by at most their magnitudes times 2^-52 times
+    # the additions along one chain of partial sums, here counted as 2000
+    most = (np.abs((h - y) * times)) @ np.abs(Q)
+    assert (np.abs(g - want) <= 2000 * 2.0 ** -52 * most).all()
