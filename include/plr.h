@@ -392,9 +392,10 @@ int plr_probe_copy_bandwidth(plr_ctx* ctx, int64_t bytes, int reps, double* gb_p
 const char* plr_kernel_info(const plr_ctx* ctx);
 
 /* Context-owned message of the last error ("" if none); never freed.
- * plr_last_error(NULL) describes the last failure of a call that takes no
- * context (plr_create, plr_loss_grad_noalloc, the plr_mxfp_* calls and
- * plr_dropout_apply). */
+ * plr_last_error(NULL) describes the calling thread's last failure of a call
+ * that takes no context (plr_create, plr_loss_grad_noalloc, the plr_mxfp_*
+ * calls and plr_dropout_apply); a thread that has had none reads the process's
+ * last one.  That text stays as it is until the thread's next such call. */
 const char* plr_last_error(const plr_ctx* ctx);
 
 const char* plr_version(void);

@@ -184,7 +184,24 @@ const PairVariant kPair = {8, 4, {plr::pair_pass<8, 4, 2, false>, plr::pair_pass
 // the column-blocked path's shape: 8 waves x 16 chunks, one row per tile, theta in LDS
 const Shape kBlockShape = {kBlkNch, 1, kBlkWcol, 1, 2, true, 0};
 
-std::string g_create_error;  // last failure of a call that has no context
+// What plr_last_error(NULL) tells: the calling thread's last failure of a call that takes no
+// context (calls that overlap each read their own, and nothing another thread does can move the
+// text), or the process's last one where this thread has had none.
+struct ErrorText {
+  char text[512];
+};
+thread_local ErrorText t_error = {};
+thread_local bool t_failed = false;
+ErrorText g_last_error = {};
+std::mutex g_err_mutex;  // g_last_error is shared by every thread
+
+int fail_without_context(int code, const char* msg) {
+  snprintf(t_error.text, sizeof t_error.text, "%s", msg);
+  t_failed = true;
+  std::lock_guard<std::mutex> lock(g_err_mutex);
+  g_last_error = t_error;
+  return code;
+}
 
 // ---- static device scratch of plr_loss_grad_noalloc ------------------------
 // Everything that entry point needs beyond the caller's inputs and outputs:
@@ -211,7 +228,6 @@ int g_na_num_cu[kNaMaxDevices] = {};
 // workgroups per compute unit of the variant for a pitch of k chunks, per
 // device (0: not asked yet): the occupancy query runs once per (device, pitch)
 int g_na_occ[kNaMaxDevices][kNaMaxPitch / plr::kChunkCols + 1] = {};
-std::mutex g_err_mutex;  // g_create_error is shared by every context-free call
 
 // Shard held in 4 bits.  Narrow rows are read once, theta and a tile's partial dot products in LDS;
 // wide ones go in column pieces, in two sweeps, where no wave waits for a whole row.
@@ -266,14 +282,7 @@ const PackedSweep kAxpy = {kAxpyPiece, {make_axpy<8, 768, 3, false>(), make_axpy
 
 }  // namespace
 
-int plr_fail_without_context(int code, const char* msg) {
-  try {
-    std::lock_guard<std::mutex> lock(g_err_mutex);
-    g_create_error = msg;
-  } catch (...) {
-  }
-  return code;
-}
+int plr_fail_without_context(int code, const char* msg) { return fail_without_context(code, msg); }
 
 struct PackedLaunch {
   const PackedFns* fns = nullptr;
@@ -1302,10 +1311,7 @@ int run_pass(plr_ctx* c, PassKind kind, const double* theta, unsigned loss_mode,
 extern "C" {
 
 int plr_create(plr_ctx** out, int device_id) {
-  auto set_err = [](const std::string& m) {
-    std::lock_guard<std::mutex> lock(g_err_mutex);
-    g_create_error = m;
-  };
+  auto set_err = [](const std::string& m) { fail_without_context(PLR_ERR_HIP, m.c_str()); };
   if (!out) {
     set_err("out must not be NULL");
     return PLR_ERR_INVALID;
@@ -2561,9 +2567,7 @@ int plr_loss_grad_noalloc(int device_id, void* hip_stream, const double* dX, con
                           int64_t n, int64_t d, int64_t ldx, const double* dtheta,
                           double* dout, unsigned flags) {
   auto bad = [](int code, const std::string& msg) {
-    std::lock_guard<std::mutex> lock(g_err_mutex);
-    g_create_error = "plr_loss_grad_noalloc: " + msg;
-    return code;
+    return fail_without_context(code, ("plr_loss_grad_noalloc: " + msg).c_str());
   };
   if (device_id < 0 || device_id >= kNaMaxDevices) return bad(PLR_ERR_INVALID, "device_id out of range");
   if (n < 0 || d < 1) return bad(PLR_ERR_INVALID, "need n >= 0 and d >= 1");
@@ -2738,7 +2742,12 @@ int plr_loss_grad_noalloc(int device_id, void* hip_stream, const double* dX, con
 const char* plr_kernel_info(const plr_ctx* c) { return c ? c->info.c_str() : ""; }
 
 const char* plr_last_error(const plr_ctx* c) {
-  return c ? c->err.c_str() : g_create_error.c_str();
+  if (c) return c->err.c_str();
+  if (!t_failed) {
+    std::lock_guard<std::mutex> lock(g_err_mutex);
+    t_error = g_last_error;
+  }
+  return t_error.text;
 }
 
 const char* plr_version(void) { return "plr 0.1 (gfx950)"; }

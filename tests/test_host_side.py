@@ -1,0 +1,89 @@
+"""The library's host side on a runtime without a device (hip_stub.cpp): calls that overlap, calls
+that fail half way, and what is launched.  Each check runs in a process of its own, which loads the
+stand-in in place of the HIP runtime."""
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+
+PRELUDE = """
+import ctypes as C, sys, threading
+stub = C.CDLL({stub!r}, mode=C.RTLD_GLOBAL)
+stub.stub_launch.restype = C.c_char_p
+for f in (stub.stub_calls, stub.stub_live, stub.stub_launches):
+    f.restype = C.c_long
+for f in (stub.stub_launch, stub.stub_fail_at):
+    f.argtypes = [C.c_long]
+sys.path[:0] = [{root!r}, {here!r}]
+import numpy as np
+from paracel_amd import Plr, PlrError, capi
+capi.load_library()
+P = 1 << 20  # stands for an aligned device address
+
+def launches():
+    out = [stub.stub_launch(i).decode() for i in range(stub.stub_launches())]
+    stub.stub_clear()
+    return out
+"""
+
+
+@pytest.fixture(scope="module")
+def check(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("stub") / "hip_stub.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
+                    "-I", os.path.join(ROCM, "include"), "-Wl,-soname,libamdhip64.so.7", "-o", so,
+                    os.path.join(HERE, "hip_stub.cpp")], check=True)
+
+    def run(body):
+        code = PRELUDE.format(stub=so, root=os.path.dirname(HERE), here=HERE) + textwrap.dedent(body)
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110)
+        assert r.returncode == 0, r.stdout + r.stderr
+        return r.stdout
+
+    return run
+
+
+def test_each_thread_reads_its_own_failure(check):
+    check("""
+        wrong = []
+
+        def work(what, f, *a):
+            for _ in range(4000):
+                try:
+                    f(*a)
+                except PlrError as e:
+                    if what not in str(e):
+                        wrong.append((what, str(e)))
+
+        jobs = [("unknown element type", capi.mxfp_quantize, P, 9, 5, 100, 100, P, 64, P, 4),
+                ("drop must not be NULL", capi.dropout_apply, P, 1, 5, 100, 100, P, 100, None),
+                ("ldo must be", capi.mxfp_dequantize, P, 64, P, 4, 5, 100, P, 1, 99),
+                ("exceeds", capi.loss_grad_noalloc, P, P, 4, 100, 1 << 20, P, P)]
+        threads = [threading.Thread(target=work, args=j) for j in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong, (len(wrong), wrong[0])
+    """)
+
+
+def test_a_failure_in_another_thread_is_still_told(check):
+    # a thread without a failure of its own reads the process's last one
+    check("""
+        def fail():
+            try:
+                Plr(99)
+            except PlrError:
+                pass
+
+        t = threading.Thread(target=fail)
+        t.start()
+        t.join()
+        assert "device_id out of range" in capi.load_library().plr_last_error(None).decode()
+    """)
