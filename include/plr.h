@@ -291,7 +291,10 @@ int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned 
  * reads 17/32 of a byte per value instead of 8.  A constant first column that
  * is not stored ("first_column_is_one") stays exact.  plr_get_data returns the
  * rounded values; plr_set_data_chunk is refused until the next plr_set_data /
- * plr_alloc_data, which starts a shard of doubles again. */
+ * plr_alloc_data, which starts a shard of doubles again.
+ * The doubles, the codes and a pass's workspace are resident together while
+ * the call runs; when it fails (PLR_ERR_NOMEM, say) the doubles stay as they
+ * were. */
 int plr_pack_data(plr_ctx* ctx);
 
 /* Dropout of the shard's values in the passes that make a gradient

@@ -429,31 +429,31 @@ void release_upload_staging(plr_ctx* c) {
   c->up_dev = nullptr;
 }
 
-void free_shape(plr_ctx* c) {
+// What the resident shard holds, given back ...
+void release_shape(plr_ctx* c) {
   (void)hipSetDevice(c->device);
   release_upload_staging(c);
-  if (c->dX) (void)hipFree(c->dX);
-  if (c->d_codes) (void)hipFree(c->d_codes);
-  if (c->d_marks) (void)hipFree(c->d_marks);
-  c->d_marks = nullptr;
-  if (c->d_scales) (void)hipFree(c->d_scales);
+  for (void* p : {(void*)c->dX, (void*)c->d_codes, (void*)c->d_scales, (void*)c->d_marks, (void*)c->dy,
+                  (void*)c->d_theta, (void*)c->d_part_g, (void*)c->d_part_loss, (void*)c->d_part_res,
+                  (void*)c->d_h, (void*)c->d_curve, (void*)c->d_zx, (void*)c->d_z, (void*)c->d_zparts,
+                  (void*)c->d_res, (void*)c->d_train_out})
+    if (p) (void)hipFree(p);
+  for (void* p : {(void*)c->h_pred, (void*)c->h_theta, (void*)c->h_out})
+    if (p) (void)hipHostFree(p);
+}
+// ... and everything that belongs to it as in a context without one.
+void forget_shape(plr_ctx* c) {
+  c->up_dev = nullptr;
+  c->dX = c->dy = c->d_theta = c->d_part_g = c->d_part_loss = c->d_part_res = c->d_h = c->d_curve = c->d_z =
+      c->d_zparts = c->d_res = c->d_train_out = nullptr;
+  c->h_theta = c->h_theta_dev = c->h_out = c->h_out_dev = c->h_pred = c->h_pred_dev = nullptr;
   c->d_codes = c->d_scales = nullptr;
+  c->d_marks = nullptr;
+  c->d_zx = nullptr;
   c->packed = c->packed_sweeps = false;
   c->row_blocks = 0;
-  if (c->dy) (void)hipFree(c->dy);
-  if (c->d_theta) (void)hipFree(c->d_theta);
-  if (c->d_part_g) (void)hipFree(c->d_part_g);
-  if (c->d_part_loss) (void)hipFree(c->d_part_loss);
-  if (c->d_part_res) (void)hipFree(c->d_part_res);
-  c->d_part_res = nullptr;
   c->bias = false;
   c->dcols = 0;
-  if (c->d_h) (void)hipFree(c->d_h);
-  if (c->h_pred) (void)hipHostFree(c->h_pred);
-  c->h_pred = c->h_pred_dev = nullptr;
-  if (c->d_curve) (void)hipFree(c->d_curve);
-  if (c->d_zx) (void)hipFree(c->d_zx);
-  c->d_zx = nullptr;
   c->team_blocks = c->team_blk_chunks = c->team_blk_extra = c->team_nch = c->nteams = 0;
   c->team_fns = nullptr;
   c->zx_words = 0;
@@ -463,15 +463,6 @@ void free_shape(plr_ctx* c) {
   c->sweep_grid = 0;
   c->part_rows = c->part_len = 0;
   c->base_info.clear();
-  if (c->d_z) (void)hipFree(c->d_z);
-  if (c->d_zparts) (void)hipFree(c->d_zparts);
-  c->d_zparts = nullptr;
-  if (c->d_res) (void)hipFree(c->d_res);
-  if (c->d_train_out) (void)hipFree(c->d_train_out);
-  if (c->h_theta) (void)hipHostFree(c->h_theta);
-  if (c->h_out) (void)hipHostFree(c->h_out);
-  c->dX = c->dy = c->d_theta = c->d_part_g = c->d_part_loss = c->d_h = c->d_curve = c->d_z = c->d_res =
-      c->d_train_out = c->h_theta = c->h_theta_dev = c->h_out = c->h_out_dev = nullptr;
   c->n = c->d = c->pitch = 0;
   c->have_data = false;
   c->curve_len = 0;
@@ -483,6 +474,10 @@ void free_shape(plr_ctx* c) {
   c->var = nullptr;
   c->fns = nullptr;
   c->info.clear();
+}
+void free_shape(plr_ctx* c) {
+  release_shape(c);
+  forget_shape(c);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1947,17 +1942,14 @@ int plr_pack_data(plr_ctx* c) {
     }
     PLR_HIP(c, hipStreamSynchronize(c->stream));
   }
-  // from here on the doubles are gone: the shard is the packed one, or none
-  const bool bias = c->bias;
-  const int64_t dcols = c->dcols;
-  double* const y = c->dy;
-  c->dy = nullptr;
-  free_shape(c);
+  // The packed shard is made ready beside the doubles, which go only when nothing can fail any more.
+  plr_ctx doubles = *c;
+  forget_shape(c);
   c->n = n;
   c->d = d;
-  c->bias = bias;
-  c->dcols = dcols;
-  c->dy = y;
+  c->bias = doubles.bias;
+  c->dcols = doubles.dcols;
+  c->dy = doubles.dy;
   c->packed = true;
   c->d_codes = static_cast<uint8_t*>(codes.p);
   c->d_scales = static_cast<uint8_t*>(scales.p);
@@ -1965,7 +1957,15 @@ int plr_pack_data(plr_ctx* c) {
   int rc = plan_packed(c, n);
   c->bias_slot = c->theta_len;
   if (rc == PLR_OK) rc = alloc_workspace(c);
-  if (rc != PLR_OK) free_shape(c);  // keeps c->err
+  if (rc == PLR_OK) {
+    doubles.dy = nullptr;  // kept
+    release_shape(&doubles);
+  } else {
+    doubles.err = c->err;
+    c->dy = nullptr;
+    release_shape(c);
+    *c = doubles;
+  }
   return rc;
 }
 

@@ -87,3 +87,42 @@ def test_a_failure_in_another_thread_is_still_told(check):
         t.join()
         assert "device_id out of range" in capi.load_library().plr_last_error(None).decode()
     """)
+
+
+@pytest.mark.parametrize("n, d, first", [(50, 100, 0), (40, 20, 0), (60, 70, 0), (30, 16400, 0), (20, 20000, 0),
+                                         (33, 258, 1), (0, 40, 0)])
+def test_packing_that_fails_leaves_the_shard(check, n, d, first):
+    check(f"""
+        n, d = {n}, {d}
+        X, y, theta = np.ones((n, d)), np.zeros(n), np.ones(d)
+        k = 0
+        while True:
+            k += 1
+            p = Plr(0)
+            p.set_option("first_column_is_one", {first})
+            p.set_data(X, y)
+            info = p.kernel_info()
+            stub.stub_fail_at(k)
+            try:
+                p.pack_data()
+                done = stub.stub_calls() < k
+            except PlrError as e:
+                done = False
+                assert e.code in (-2, -3) and "out of memory" in str(e), (e.code, str(e))
+                stub.stub_fail_at(0)
+                # the doubles are resident as before, and pack when asked again
+                assert p.kernel_info() == info, (k, p.kernel_info())
+                rows, cols = C.c_int64(), C.c_int64()
+                p._lib.plr_get_shape(p._h, C.byref(rows), C.byref(cols))
+                assert (rows.value, cols.value) == (n, d)
+                p.loss_grad(theta)
+                p.pack_data()
+            stub.stub_fail_at(0)
+            assert "4-bit" in p.kernel_info()
+            p.loss_grad(theta)
+            p.close()
+            assert stub.stub_live() == 0, (k, stub.stub_live())
+            if done:
+                break
+        assert k > 5
+    """)
