@@ -294,7 +294,8 @@ int plr_dropout_apply(int device_id, void* hip_stream, const void* dx, unsigned 
  * plr_alloc_data, which starts a shard of doubles again.
  * The doubles, the codes and a pass's workspace are resident together while
  * the call runs; when it fails (PLR_ERR_NOMEM, say) the doubles stay as they
- * were. */
+ * were.  Rows of more than 268431360 stored columns are refused with
+ * PLR_ERR_UNSUPPORTED. */
 int plr_pack_data(plr_ctx* ctx);
 
 /* Dropout of the shard's values in the passes that make a gradient

@@ -265,6 +265,7 @@ constexpr int kPackedFused[3] = {128, 256, 64};
 // second one side by side in one workgroup, whose sums then leave it as one (12000 x 16385: three
 // workgroups of 256 threads 81 us a pass, one of 768 79; 3000 x 40001: 72 and 57).
 constexpr int kDotPiece = 128, kAxpyPiece = 256, kSweepSlots = 64;
+constexpr int kMostPieces = 65535;  // of a row: they are a grid's y
 struct PackedSweep {
   int most_blocks;  // of a piece
   PackedFns fns[2];  // [dropout]
@@ -701,7 +702,7 @@ int plan_packed_launch(plr_ctx* c, const PackedFns* f, int64_t n, int64_t piece,
 // (513 blocks in pieces of 256, 256 and 1 take a round of workgroups more than in 9 of 57).
 int plan_packed_sweep(plr_ctx* c, const PackedSweep& s, bool drop, int64_t n, PackedLaunch* best) {
   const int64_t least = ceil_div(c->row_blocks, s.most_blocks);
-  for (int64_t pieces = least; pieces <= least + 8; ++pieces) {
+  for (int64_t pieces = least; pieces <= std::min<int64_t>(least + 8, kMostPieces); ++pieces) {
     PackedLaunch l;
     const int rc = plan_packed_launch(c, &s.fns[drop], n, ceil_div(c->row_blocks, pieces), false, &l);
     if (rc != PLR_OK) return rc;
@@ -1907,10 +1908,12 @@ int plr_pack_data(plr_ctx* c) {
   if (!c) return PLR_ERR_INVALID;
   if (!c->have_data) return fail(c, PLR_ERR_NODATA, "no shard resident: call plr_set_data first");
   if (c->packed) return PLR_OK;
+  const int64_t n = c->n, d = c->d, blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
+  if (blocks > (int64_t)kMostPieces * kDotPiece)
+    return fail(c, PLR_ERR_UNSUPPORTED, "rows of more than 268431360 stored columns are not held in 4 bits");
   PLR_HIP(c, hipSetDevice(c->device));
   PLR_HIP(c, hipStreamSynchronize(c->stream));
   release_upload_staging(c);
-  const int64_t n = c->n, d = c->d, blocks = ceil_div(c->dcols, plr_mx::kBlockCols);
   DevBuf codes, scales;
   if (n > 0) {
     // zeros behind the last row, which the kernels read

@@ -118,6 +118,9 @@ hipError_t __hipPopCallConfiguration(dim3* grid, dim3* block, size_t* lds, hipSt
   return hipSuccess;
 }
 hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void**, size_t, hipStream_t) {
+  // a launch counts its threads in 32 bits, and its workgroups down and behind in 16
+  if ((unsigned long long)grid.x * block.x > 0xffffffffull || grid.y > 65535 || grid.z > 65535)
+    return done(hipErrorInvalidConfiguration);
   char b[128];
   snprintf(b, sizeof b, " %u %u %u %u", grid.x, grid.y, grid.z, block.x * block.y * block.z);
   std::lock_guard<std::mutex> l(g_lock);

@@ -126,3 +126,25 @@ def test_packing_that_fails_leaves_the_shard(check, n, d, first):
                 break
         assert k > 5
     """)
+
+
+def test_the_widest_rows(check):
+    # the first sweep takes a row in pieces of 128 blocks, a workgroup down the grid to each
+    check("""
+        most = 65535 * 128 * 32
+        p = Plr(0)
+        p.alloc_data(1, most + 1)
+        info = p.kernel_info()
+        try:
+            p.pack_data()
+            assert False, p.kernel_info()
+        except PlrError as e:
+            assert e.code == -5 and str(most) in str(e), str(e)
+        assert p.kernel_info() == info
+        p.close()
+        p = Plr(0)
+        p.alloc_data(1, most)
+        p.pack_data()
+        p.calc_loss(np.zeros(most))
+        assert any("packed_pass" in l and " 65535 " in l for l in launches())
+    """)
