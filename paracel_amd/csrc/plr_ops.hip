@@ -591,6 +591,7 @@ struct Call {
     stream = reinterpret_cast<hipStream_t>(hip_stream);
     if (device_id < 0 || device_id >= kMaxDevices)
       return bad(PLR_ERR_INVALID, "device_id out of range");
+    (void)hipGetLastError();  // what the caller left behind is not this call's (launched())
     int cur = -1;
     hipError_t e = hipGetDevice(&cur);
     if (e != hipSuccess) return hip(e, "hipGetDevice");

@@ -148,3 +148,17 @@ def test_the_widest_rows(check):
         p.calc_loss(np.zeros(most))
         assert any("packed_pass" in l and " 65535 " in l for l in launches())
     """)
+
+
+def test_an_error_left_behind_is_not_the_calls_own(check):
+    # the caller's earlier failure (600: an event that was not ready) is still its thread's last error
+    check("""
+        drop = capi.Dropout(0.5, 1)
+        for call in (lambda: capi.mxfp_quantize(P, 1, 5, 100, 100, P, 64, P, 4),
+                     lambda: capi.mxfp_dequantize(P, 64, P, 4, 5, 100, P, 1, 100),
+                     lambda: capi.dropout_apply(P, 1, 5, 100, 100, P, 100, drop),
+                     lambda: capi.mxfp_matmul(5, 7, 100, P, 64, P, 4, P, 64, P, 4, P, 1, 7)):
+            stub.stub_error(600)
+            call()
+            assert len(launches()) == 1
+    """)
