@@ -6,6 +6,7 @@
 //   stub_live()       allocations not freed yet
 //   stub_launches()   launches recorded since stub_clear(); stub_launch(i) names one:
 //                     "kernel<arguments> x y z threads"
+//   stub_kernels()    kernels the library has; stub_kernel(i) names one
 //   stub_error(e)     leaves e behind as the calling thread's last error
 #include <cxxabi.h>
 #include <hip/hip_runtime_api.h>
@@ -13,6 +14,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <iterator>
 #include <map>
 #include <mutex>
 #include <string>
@@ -72,6 +74,8 @@ void stub_clear() {
 }
 long stub_launches() { return (long)g_launches.size(); }
 const char* stub_launch(long i) { return g_launches[i].c_str(); }
+long stub_kernels() { return (long)g_names.size(); }
+const char* stub_kernel(long i) { return std::next(g_names.begin(), i)->second.c_str(); }
 
 void** __hipRegisterFatBinary(const void*) {
   static void* module;

@@ -1,0 +1,92 @@
+"""The product's tiles over many steps of k, its strips beside a multiple of the tile, and the
+transposed quantiser's own rounding.  PATHS is chosen by which kernels a product of these sizes is
+cut into on a device of 256 compute units; test_host_side.py checks without a GPU that every
+kernel of the product is reached by it and by test_gpu_mxfp.MATMULS."""
+import numpy as np
+import pytest
+
+import mxfp_ref as ref
+from test_gpu_mxfp import NAMES, _bound, _matmul, device_codes, features
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def capi():
+    from paracel_amd import capi
+
+    capi.load_library()
+    return capi
+
+
+# m, n, k, type.  Steps of 128 along k: 13 to 17 and more, so that the ring of four stages, the
+# groups of four steps with every remainder and the ring of three groups of scales are gone round.
+PATHS = [
+    (2300, 4090, 1800, 1),  # tiles of 256 x 256, ragged; 15 steps
+    (4094, 4138, 1750, 2),  # ... and a strip of 42 columns; 14
+    (4120, 4093, 2000, 3),  # ... and of 24 rows; 16
+    (4140, 4120, 2100, 2),  # ... and both; 17
+    (2000, 4060, 2700, 2),  # tiles of 128 x 256; 22
+    (4100, 2048, 2690, 1),  # ... and a strip of 4 rows; 22
+    (1063, 1021, 2031, 3),  # tiles of 128 x 128; 16
+    (1545, 2546, 1596, 2),  # ... and a strip of 9 rows; 13
+    (2995, 1312, 1953, 1),  # ... and of 32 columns; 16
+    # few rows on one side, and small products, in the kernels' other forms
+    (700, 9, 2100, 2), (30, 9000, 300, 3), (9000, 30, 300, 1), (9000, 40, 260, 2), (600, 500, 1500, 3),
+]
+
+
+@pytest.mark.parametrize("m, n, k, dtype", PATHS)
+def test_matmul_paths(capi, m, n, k, dtype):
+    rng = np.random.default_rng(m + n + k)
+    a, b = ref.quantize(features(rng, m, k) / 16), ref.quantize(rng.normal(size=(n, k)) / 16)
+    va, vb = ref.values(*a)[:, :k], ref.values(*b)[:, :k]
+    want = 0.75 * (va @ vb.T)
+    bound = _bound(va, vb, k, want, dtype, 0.75)
+    got = _matmul(capi, a, b, k, dtype, 0.75, pad=1, ldc=n + 3)
+    assert (np.abs(got - want) <= bound).all()
+    # the mask of the result: rows and columns of the strips are those of the whole
+    drop = capi.Dropout(0.5, 0x1234567887654321, 5, (1 << 32) - 1000)  # factor 2: exact
+    keep = ref.keep(m, n, drop)
+    got = _matmul(capi, a, b, k, dtype, 0.75, drop, ldc=-(-n // 8) * 8)
+    assert (got[~keep] == 0).all()
+    # twice the value, and twice its bound but for the type's smallest step, which is in it once
+    assert (np.abs(got - 2 * want) <= 2 * bound)[keep].all()
+
+
+@pytest.mark.parametrize("dtype", range(4), ids=NAMES)
+def test_quantize_edges_along_columns(capi, dtype):
+    # the values of test_quantize_edges as columns of x: every one of them passes through the columns
+    # that are taken 16 bytes at a time and through the ones behind the last whole 16 bytes, in a
+    # whole block of 32 rows in front of one that ends early
+    tiny = [2.0 ** -1074, 2.0 ** -149, 2.0 ** -133, 2.0 ** -24][dtype]
+    big = [np.finfo(np.float64).max, np.finfo(np.float32).max, 3.3895313892515355e38, 65504.0][dtype]
+    cols = [np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -0.25, -0.75, -5.0, 4.0] * 3)[:32],
+            np.full(32, tiny), np.r_[big, np.full(31, tiny)], np.r_[-big, np.zeros(31)],
+            np.zeros(32), -np.zeros(32), np.r_[np.nan, np.ones(31)], np.r_[np.ones(31), np.inf],
+            np.r_[np.ones(31), -np.inf], np.r_[2.0 ** -14, np.full(31, 2.0 ** -16)],
+            np.linspace(-8, 8, 32)]
+    if dtype == 0:
+        cols.append(np.r_[6.0, np.full(10, 0.25 * (1 + 2.0 ** -50)), np.full(10, 2.5 * (1 - 2.0 ** -50)),
+                          np.full(11, 3.5 * (1 - 2.0 ** -52))])
+    v = 16 // [8, 4, 2, 2][dtype]
+    while len(cols) % v != v - 1:
+        cols.append(np.full(32, 1.5))
+    cols = [np.r_[c, c[:5]] for c in cols]
+    for turn in range(len(cols)):
+        x = ref.store(np.array(cols[turn:] + cols[:turn]).T, dtype)
+        for drop in (None, capi.Dropout(0.5, turn)):
+            w = np.where(ref.keep(*x.shape, drop), ref.load(x, dtype), 0.0)
+            _same_codes(device_codes(capi, x, dtype, True, drop), *ref.quantize(w.T))
+
+
+def _same_codes(got, code, s):
+    want = ref.pack(code, s, got[0].shape[1], got[1].shape[1])
+    n = code.shape[0]
+
+    def plus(a):  # a code of minus zero stands for the value plus zero does
+        a = np.where((a & 0x0F) == 8, a & 0xF0, a)
+        return np.where((a & 0xF0) == 0x80, a & 0x0F, a)
+
+    assert np.array_equal(got[1][:n], want[1])
+    assert np.array_equal(plus(got[0][:n]), plus(want[0]))

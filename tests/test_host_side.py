@@ -14,10 +14,10 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 PRELUDE = """
 import ctypes as C, sys, threading
 stub = C.CDLL({stub!r}, mode=C.RTLD_GLOBAL)
-stub.stub_launch.restype = C.c_char_p
-for f in (stub.stub_calls, stub.stub_live, stub.stub_launches):
+stub.stub_launch.restype = stub.stub_kernel.restype = C.c_char_p
+for f in (stub.stub_calls, stub.stub_live, stub.stub_launches, stub.stub_kernels):
     f.restype = C.c_long
-for f in (stub.stub_launch, stub.stub_fail_at):
+for f in (stub.stub_launch, stub.stub_kernel, stub.stub_fail_at):
     f.argtypes = [C.c_long]
 sys.path[:0] = [{root!r}, {here!r}]
 import numpy as np
@@ -161,4 +161,30 @@ def test_an_error_left_behind_is_not_the_calls_own(check):
             stub.stub_error(600)
             call()
             assert len(launches()) == 1
+    """)
+
+
+def test_the_products_tested_reach_every_kernel(check):
+    # the shapes of the GPU tests: every kernel of the product that the library has (in one of its
+    # three result types, with and without dropout; a shape is tested both ways), every size of
+    # tile over long k with rows or with columns over, and groups of four steps with every remainder
+    check("""
+        import test_gpu_mxfp, test_gpu_mxfp_paths
+        reached, over, steps = set(), set(), {}
+        short = lambda k: k.split("matmul_")[1].split(">")[0].replace("<bfloat16, false, ", "<")
+        for m, n, k in test_gpu_mxfp.MATMULS + [c[:3] for c in test_gpu_mxfp_paths.PATHS]:
+            p, q = capi.mxfp_code_pitch(k), capi.mxfp_scale_pitch(k)
+            capi.mxfp_matmul(m, n, k, P, p, P, q, P, p, P, q, P, 2, n)
+            got = [short(l) for l in launches()]
+            reached.update(got)
+            if "tiles" in got[0] and k > 12 * 128:
+                over.update((got[0], l.split(", ")[-1]) for l in got[1:])
+                steps.setdefault(got[0], set()).add(-(-k // 128) % 4)
+        kernels = [stub.stub_kernel(i).decode() for i in range(stub.stub_kernels())]
+        kernels = {short(k) for k in kernels if "matmul_" in k and "<bfloat16, false, " in k}
+        assert kernels and not kernels - reached, kernels - reached
+        assert len(steps) == len([k for k in kernels if "tiles" in k]) == 3
+        assert {0, 1, 2, 3} in steps.values()
+        assert {t for t, _ in over} == set(steps)  # strips of rows (false) and of columns (true)
+        assert {s for _, s in over} == {"false", "true"}
     """)
