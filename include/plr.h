@@ -256,8 +256,10 @@ int plr_mxfp_dequantize(int device_id, void* hip_stream, const uint8_t* dcodes, 
                         unsigned type, int64_t ldo);
 
 /* C[i][j] = alpha * sum_k A[i][k] * B[j][k], A of m rows and B of n rows of k
- * columns in 4 bits, the sums in 32 bits, C of `type` (PLR_F32, PLR_BF16 or
- * PLR_F16) at a row pitch of ldc values.  The scores of m samples under n
+ * columns in 4 bits, the sums and alpha (times the mask's factor) in 32 bits,
+ * C of `type` (PLR_F32, PLR_BF16 or PLR_F16) at a row pitch of ldc values.  An
+ * alpha that is finite and not 0 must, times that factor, be a normal number
+ * of 32 bits: magnitudes of 2^-126 to 2^128.  The scores of m samples under n
  * coefficient vectors, next to plr_predict_linear's one; with
  * PLR_MXFP_TRANSPOSE operands also both gradients of such a product:
  * dA = dC B as quantise(dC) . quantise(B, transposed) and dB = dC^T A as

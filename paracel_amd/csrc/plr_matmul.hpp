@@ -22,8 +22,7 @@ struct MatmulArgs {
   int chunks;  // of 128 values along k
   void* c;
   int64_t ldc;
-  float alpha;
-  float kept;  // dropout: the factor of what is kept
+  float factor;  // alpha times what the mask multiplies kept values by
   int64_t row0, col0;  // where c's first element stands in the matrix that the mask belongs to
   Mask mask;
 };
@@ -63,8 +62,8 @@ __device__ __forceinline__ Out8<T> finish8(const MatmulArgs& p, int64_t i, int64
   Out8<T> o;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float v = p.alpha * (e < 4 ? lo[e & 3] : hi[e & 3]);
-    if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * p.kept;
+    float v = p.factor * (e < 4 ? lo[e & 3] : hi[e & 3]);
+    if (DROP && (drops >> 4 * e & 1)) v = 0.f;
     o.v[e] = (T)v;
   }
   return o;
@@ -430,10 +429,10 @@ __global__ __launch_bounds__(64 * W) void matmul_few(FewArgs a) {
       T out[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = a.p.alpha * acc[x][y][e];
+        float v = a.p.factor * acc[x][y][e];
         if (DROP && SWAP)
           drops = drop_marks(a.p.mask, xr + e + a.p.row0, (unsigned)((yr + a.p.col0) >> 3)) >> 4 * (yr & 7) << 4 * e;
-        if (DROP) v = (drops >> 4 * e & 1) ? 0.f : v * a.p.kept;
+        if (DROP && (drops >> 4 * e & 1)) v = 0.f;
         out[e] = (T)v;
       }
       T* c = static_cast<T*>(a.p.c);

@@ -5,6 +5,7 @@
 #include "../../include/plr.h"
 
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdio.h>
 #include <string.h>
@@ -902,6 +903,11 @@ int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64
   double scale;
   int rc = check_mask(c, drop, &a.mask, &scale);
   if (rc != PLR_OK) return rc;
+  // One factor for alpha and the mask, rounded to 32 bits once (2^-24): two multiplications could pass
+  // through a number too small for 32 bits on the way to one that is not.
+  const double factor = alpha * scale;
+  if (alpha != 0. && isfinite(alpha) && !(fabs(factor) >= FLT_MIN && fabs(factor) <= FLT_MAX))
+    return c.bad(PLR_ERR_INVALID, "alpha times the mask's factor must be 0 or a normal number of 32 bits");
   if (workspace_bytes < plr_mxfp_matmul_workspace(m, n, k))
     return c.bad(PLR_ERR_INVALID, "workspace smaller than plr_mxfp_matmul_workspace(m, n, k)");
   (void)workspace;  // none of the kernels asks for any
@@ -925,8 +931,7 @@ int plr_mxfp_matmul(int device_id, void* hip_stream, int64_t m, int64_t n, int64
   a.chunks = (int)ceil_div(k, 128);
   a.c = dc;
   a.ldc = ldc;
-  a.alpha = (float)alpha;
-  a.kept = (float)scale;
+  a.factor = (float)factor;
   a.row0 = a.col0 = 0;
   rc = c.begin(device_id, hip_stream);
   if (rc != PLR_OK || m == 0 || n == 0) return rc;

@@ -90,3 +90,17 @@ def _same_codes(got, code, s):
 
     assert np.array_equal(got[1][:n], want[1])
     assert np.array_equal(plus(got[0][:n]), plus(want[0]))
+
+
+def test_factor_of_a_dropped_product(capi):
+    # 2^-30 times these sums is below the smallest normal number of 32 bits, times the mask's
+    # factor it is not: the two are joined before the sum is rounded.  Everything is exact.
+    drop = capi.Dropout(1 - 2.0 ** -8, 3, 1, 9)  # factor 256
+    for m, n, k in ((16, 20000, 64), (30, 9000, 64), (500, 600, 64), (1063, 1021, 2031), (2300, 4090, 1800)):
+        x, y = np.zeros((m, k)), np.zeros((n, k))
+        x[:, 0], y[:, 0] = 2.0 ** -50, 2.0 ** -50
+        x[:, 32], y[:, 32] = 2.0 ** -60, 2.0 ** -61
+        got = _matmul(capi, ref.quantize(x), ref.quantize(y), k, 1, 2.0 ** -30, drop)
+        keep = ref.keep(m, n, drop)
+        assert keep.any()
+        assert (got == np.where(keep, 2.0 ** -122 + 2.0 ** -143, 0)).all()

@@ -144,3 +144,10 @@ def test_context_calls_refuse_null(capi):
     lib = capi.load_library()
     assert lib.plr_pack_data(None) == -1
     assert lib.plr_set_dropout(None, C.byref(capi.Dropout(0.5, 1))) == -1
+
+
+@pytest.mark.parametrize("alpha, rate", [(1e300, 0), (-1e39, 0), (1e-40, 0), (1e-320, 0), (-1e-39, 0.5),
+                                         (1e34, 65535 / 65536)])
+def test_matmul_refuses_factors_that_32_bits_do_not_hold(capi, alpha, rate):
+    refused("alpha", capi.mxfp_matmul, 5, 7, 100, P, 64, P, 4, P, 64, P, 4, P, 1, 7, alpha=alpha,
+            drop=capi.Dropout(rate, 1))
