@@ -3,6 +3,8 @@
 // plr_pack_data), "dropout" (the rate, default 0; needs "mxfp4") and "dropout_seed".
 #pragma once
 
+#include <errno.h>
+#include <math.h>
 #include <stdint.h>
 #include <stdlib.h>
 
@@ -26,12 +28,14 @@ struct shard_options {
     } else if (key == "dropout") {
       char* end = nullptr;
       dropout = strtod(v.c_str(), &end);
-      if (v.empty() || *end || !(dropout >= 0. && dropout < 1.))
-        throw std::invalid_argument("dropout must be a rate of at least 0 and below 1");
+      if (v.empty() || *end || !(dropout >= 0. && rint(dropout * 65536.) <= 65535.))  // as plr_set_dropout
+        throw std::invalid_argument("dropout must be a rate of at least 0 and at most 65535/65536");
     } else if (key == "dropout_seed") {
       char* end = nullptr;
+      errno = 0;
       seed = strtoull(v.c_str(), &end, 0);
-      if (v.empty() || *end) throw std::invalid_argument("dropout_seed must be a whole number");
+      if (v.empty() || v.find('-') != std::string::npos || *end || errno == ERANGE)
+        throw std::invalid_argument("dropout_seed must be a whole number from 0 to 2^64 - 1");
     }
   }
   static shard_options from(const std::map<std::string, std::string>& kv) {

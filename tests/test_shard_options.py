@@ -33,3 +33,13 @@ def test_synthetic_mode_refuses_too():
     r = subprocess.run([os.path.join(PKG, "plr_lr_worker"), "--synthetic", "1,10,10,1.0", "--dropout", "0.5"],
                        capture_output=True, text=True, timeout=60)
     assert r.returncode == 1 and "needs storage mxfp4" in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("worker", ["plr_lr_worker", "plr_ridge_worker"])
+@pytest.mark.parametrize("extra, what", [
+    # a rate that rounds to every value dropped: no pass takes it
+    ({"storage": "mxfp4", "dropout": 0.999999}, "dropout must be"),
+    ({"storage": "mxfp4", "dropout_seed": -5}, "dropout_seed must be"),
+    ({"storage": "mxfp4", "dropout_seed": 1 << 64}, "dropout_seed must be")])
+def test_values_out_of_range_are_refused(tmp_path, worker, extra, what):
+    test_refusals(tmp_path, worker, extra, what)
