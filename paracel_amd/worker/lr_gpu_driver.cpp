@@ -105,6 +105,9 @@ int main(int argc, char** argv) {
              rounds, n, d, sec, rounds / sec, kms / (rounds + 1), 1e3 * (rounds + 1) / kms, loss);
       return 0;
     }
+    if (!shard_kv.empty())
+      throw std::invalid_argument("--storage, --dropout and --dropout_seed belong to --synthetic; "
+                                  "a cfg file has keys of these names");
     auto kv = parse_flat_json(cfg_file);
     const auto shard = plr_ps::shard_options::from(kv);
     logistic_regression_gpu lr(server_info, need(kv, "training_input"), need(kv, "output"),

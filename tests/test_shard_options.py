@@ -43,3 +43,13 @@ def test_synthetic_mode_refuses_too():
     ({"storage": "mxfp4", "dropout_seed": 1 << 64}, "dropout_seed must be")])
 def test_values_out_of_range_are_refused(tmp_path, worker, extra, what):
     test_refusals(tmp_path, worker, extra, what)
+
+
+def test_flags_of_the_synthetic_mode_are_refused_beside_a_cfg_file(tmp_path):
+    # a cfg file has keys of these names; a flag beside it was not looked at
+    cfg = tmp_path / "cfg.json"
+    cfg.write_text(json.dumps(CFG))
+    for flag in (["--storage", "mxfp4"], ["--storage=mxfp4", "--dropout=0.5"], ["--dropout_seed", "3"]):
+        r = subprocess.run([os.path.join(PKG, "plr_lr_worker"), "--server_info", "", "--cfg_file", str(cfg)] + flag,
+                           capture_output=True, text=True, timeout=60)
+        assert r.returncode == 1 and "belong to --synthetic" in r.stderr, r.stderr
