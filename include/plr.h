@@ -401,7 +401,8 @@ const char* plr_kernel_info(const plr_ctx* ctx);
  * plr_last_error(NULL) describes the calling thread's last failure of a call
  * that takes no context (plr_create, plr_loss_grad_noalloc, the plr_mxfp_*
  * calls and plr_dropout_apply); a thread that has had none reads the process's
- * last one.  That text stays as it is until the thread's next such call. */
+ * last one.  That text stays as it is until the thread's next such call or its
+ * end. */
 const char* plr_last_error(const plr_ctx* ctx);
 
 const char* plr_version(void);

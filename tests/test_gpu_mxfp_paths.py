@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import mxfp_ref as ref
-from test_gpu_mxfp import NAMES, _bound, _matmul, device_codes, features
+from test_gpu_mxfp import NAMES, _bound, _check_dequantize, _matmul, device_codes, features
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +104,50 @@ def test_factor_of_a_dropped_product(capi):
         keep = ref.keep(m, n, drop)
         assert keep.any()
         assert (got == np.where(keep, 2.0 ** -122 + 2.0 ** -143, 0)).all()
+
+
+@pytest.mark.parametrize("dtype", range(4), ids=NAMES)
+@pytest.mark.parametrize("transpose", [False, True], ids=["rows", "columns"])
+def test_quantize_far_from_one(capi, dtype, transpose):
+    # magnitudes over the type's whole range, its subnormal numbers and scales of 0 and 254 among them
+    rng = np.random.default_rng(dtype)
+    low, high = [(-140, 135), (-140, 127), (-140, 127), (-24, 15)][dtype]
+    e = np.arange(low, high + 1)
+    x = rng.integers(1, 256, size=(e.size, 37)) / 256.0 * rng.choice([-1, 1], size=(e.size, 37))
+    with np.errstate(over="ignore"):
+        x = ref.store(np.ldexp(x, e[:, None] + 1), dtype)
+    v = ref.load(x, dtype)
+    assert np.isfinite(v).all()
+    if transpose:
+        x = np.ascontiguousarray(x.T)
+    _same_codes(device_codes(capi, x, dtype, transpose), *ref.quantize(v))
+
+
+@pytest.mark.parametrize("dtype", range(4), ids=NAMES)
+def test_every_code_under_every_scale(capi, dtype):
+    s = np.arange(256, dtype=np.uint8)[:, None]
+    code = np.tile(np.r_[np.arange(16), np.arange(16)[::-1]].astype(np.uint8), (256, 1))
+    with np.errstate(over="ignore"):
+        _check_dequantize(capi, code, s, 32, dtype)
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 300, 200), (40, 70, 1000), (300, 300, 600), (1063, 1021, 2031)])
+def test_matmul_of_scales_at_both_ends(capi, m, n, k):
+    # 2^-127 times 2^127, the smallest scale and the largest: exact sums of small whole numbers
+    rng = np.random.default_rng(k)
+    x, y = rng.integers(-3, 4, size=(m, k)) * 1.0, rng.integers(-3, 4, size=(n, k)) * 1.0
+    a, b = (_codes_of(v) for v in (x, y))
+    low = rng.integers(0, 255, size=a[1].shape[1])
+    low[:2] = 0, 254
+    a = (a[0], np.tile(low.astype(np.uint8), (m, 1)))
+    b = (b[0], np.tile((254 - low).astype(np.uint8), (n, 1)))
+    got = _matmul(capi, a, b, k, 1)
+    assert (got == x @ y.T).all()
+
+
+def _codes_of(v):
+    """Codes of whole numbers from -3 to 3, whatever the scale, in whole blocks."""
+    code = np.array([0, 2, 4, 5], dtype=np.uint8)[np.abs(v).astype(int)] | (v < 0).astype(np.uint8) << 3
+    out = np.zeros((v.shape[0], -(-v.shape[1] // 32) * 32), dtype=np.uint8)
+    out[:, :v.shape[1]] = code
+    return out, np.zeros((v.shape[0], out.shape[1] // 32), dtype=np.uint8)
