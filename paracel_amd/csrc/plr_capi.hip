@@ -251,8 +251,8 @@ constexpr PackedFused make_packed() {
            {STRIDE, SR, NT, NT, false, EVAL ? plr::packed_pass<false, false, plr::kPassFused, STRIDE, SR, NT, MINW> : nullptr}}};
 }
 // Row sets per tile: as many as leave two workgroups (of 512 threads one) on a compute unit; the
-// barriers and row terms of a tile cost the same however long it is (1M x 1000: 16 sets 265 us,
-// 8 sets 301).  Rows of up to 8 blocks lie 32 and more side by side: with 8 sets their partials
+// barriers and row terms of a tile cost the same however long it is (1M x 1000, 274 us: 8 sets cost
+// 14 % more).  Rows of up to 8 blocks lie 32 and more side by side: with 8 sets their partials
 // stay small enough (1M x 100 with dropout: 8 sets 80 us, 16 sets 92).
 const PackedFused kPacked[3] = {make_packed<8, 8, 256, 2, true>(), make_packed<64, 16, 256, 2, true>(),
                               make_packed<256, 8, 512, 2, false>()};
@@ -2006,10 +2006,11 @@ int plr_get_data(plr_ctx* c, int64_t row0, int64_t nrows, double* X, int64_t ldx
       if (c->packed) {
         const int rc = unpack_rows(c, row0 + r0, m, static_cast<double*>(stage.p));
         if (rc != PLR_OK) return rc;
-      } else
-      hipLaunchKernelGGL(plr::gather_rows, dim3((unsigned)ceil_div(m * d, 256)), dim3(256), 0,
-                         c->stream, (const double*)c->dX, c->pitch, c->lane ? c->lane->np : 0,
-                         row0 + r0, m, (int)d, c->bias ? 1 : 0, static_cast<double*>(stage.p));
+      } else {
+        hipLaunchKernelGGL(plr::gather_rows, dim3((unsigned)ceil_div(m * d, 256)), dim3(256), 0,
+                           c->stream, (const double*)c->dX, c->pitch, c->lane ? c->lane->np : 0,
+                           row0 + r0, m, (int)d, c->bias ? 1 : 0, static_cast<double*>(stage.p));
+      }
       PLR_HIP(c, hipGetLastError());
       PLR_HIP(c, hipStreamSynchronize(c->stream));
       if (ldx == d) {

@@ -127,7 +127,7 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned tiles_m, unsigned 
 // 64 bytes of a stage the four blocks are permuted by the row number, so that the 16 rows a wave
 // reads at once lie on different banks.
 //
-// 8192^3 in 280 us, 3.9 PFLOP/s; bound by power (the clock falls to 1.6 GHz) and by LDS: a step takes
+// 8192^3 in 271 to 280 us, 3.9 to 4.1 PFLOP/s; bound by power (the clock falls to 1.6 GHz) and by LDS: a step takes
 // 1500 cycles, the matrix instructions of its two waves per SIMD 1024.
 //
 // Scales go the same way, 16 bytes per row and group of four steps, in a ring of three groups; a
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void matmul_tiles(Ma
 // their sums meet in LDS in wave order.  Codes of four chunks are requested at once: 256 consecutive bytes of a row.  The same, in
 // pieces of 64 x 32 and 32 x 32, serves small products, which have too few large tiles to fill the
 // device.  Rows a power of two of bytes apart meet in the same channels of the L2 cache
-// (256 x 256 x 16384: 17 us, where its bytes alone are 4): 16 waves to a piece make it slower.
+// (256 x 256 x 16384: 20 us, where its bytes alone are 4): 16 waves to a piece make it slower.
 struct FewArgs {
   MatmulArgs p;
   const uint8_t *x, *y, *sx, *sy;  // many, few
@@ -470,12 +470,12 @@ inline void launch_few(const FewArgs& a, bool swap, int cus, int squares, hipStr
   const int64_t fy = (a.few + 15) / 16;
   const int64_t pieces = (a.rows + 15) / 16;
   if (fy == 1) {
-    // few workgroups: more waves of each share k (1 x 256 x 16384 9.7 us)
+    // few workgroups: more waves of each share k (1 x 256 x 16384 7.7 us)
     if (pieces < (int64_t)cus * 4 && a.p.chunks >= 16) launch_few_as<T, DROP, 1, 1, 8>(a, swap, st);
     else launch_few_as<T, DROP, 1, 1, 4>(a, swap, st);
   } else if (pieces >= (int64_t)cus * 2) {
     // two pieces of the many share what is loaded of the few, where that leaves a workgroup per
-    // compute unit (48 x 16384 x 8192: 29 us, with one piece 42; 32 x 4096 x 4096: 9.2 and 7.8)
+    // compute unit (48 x 16384 x 8192: 26 us, with one piece 38; 32 x 4096 x 4096: 6.9 and 5.7)
     if (fy == 2) launch_few_as<T, DROP, 2, 2, 4>(a, swap, st);
     else if (fy == 3) launch_few_as<T, DROP, 3, 2, 4>(a, swap, st);
     else launch_few_as<T, DROP, 4, 2, 4>(a, swap, st);
@@ -486,7 +486,7 @@ inline void launch_few(const FewArgs& a, bool swap, int cus, int squares, hipStr
   }
 }
 // Up to 32 rows always; up to 64 where tiles of 128 would leave half the device idle (48 x 16384 x
-// 8192: tiles 27 us, this 29; 33 x 9000 x 4100: 16 and 12).
+// 8192: tiles 25 us, this 26; 33 x 9000 x 4100: 12 and 10).
 inline bool few_rows(const MatmulArgs& p, int cus) {
   const int64_t few = std::min(p.m, p.n), many = std::max(p.m, p.n);
   return few <= 32 || (few <= 64 && many < (int64_t)cus * 64);
@@ -517,13 +517,14 @@ inline bool launch_few_rows(const MatmulArgs& p, int type, bool drop, int cus, i
 
 // How a product is cut up, by the microseconds each way is expected to take; constants from timing
 // all of them over sizes from 256 x 256 x 16384 to 16384 x 8192 x 4096 on an idle device of 256
-// compute units (a launch alone counts 5).  S: steps of 128 along k.
-//   tiles of 256 x 256, one to a compute unit at a time    12 + 0.89 S a round   (8192^3: 279 us)
-//   tiles of 128 x 256                                     7.6 + 0.57 S a round  (8192^3: 352)
-//   tiles of 128 x 128, two to a compute unit              3.4 + 0.74 S a round  (8192^3: 403)
+// compute units (a launch alone counts 5).  What is written of C counts nothing here: over a few steps
+// of k into a large C the choice is not borne out by timing.  S: steps of 128 along k.
+//   tiles of 256 x 256, one to a compute unit at a time    12 + 0.89 S a round   (8192^3: 271 us)
+//   tiles of 128 x 256                                     7.6 + 0.57 S a round  (8192^3: 351)
+//   tiles of 128 x 128, two to a compute unit              3.4 + 0.74 S a round  (8192^3: 397)
 //                       no more than compute units         3 + 0.27 S
 //   64 x 32 and 32 x 32 pieces straight from memory: what they load over and over, or one wave's
-//   share of k                          (512 x 512 x 8192: 19 and 14 us, tiles of 128 x 128 22)
+//   share of k                          (512 x 512 x 8192: 16 and 12 us, tiles of 128 x 128 19)
 enum Cut { kTiles256, kTiles128x256, kTiles128, kPieces64, kPieces32 };
 struct Plan {
   Cut cut;
@@ -551,7 +552,7 @@ inline bool launch_matmul(const MatmulArgs& a, int type, bool drop, int cus, hip
   if (few_rows(a, cus) && std::max(a.m, a.n) <= kMostFewRows) return launch_few_rows(a, type, drop, cus, 0, st);
   const Plan whole = plan_matmul(a.m, a.n, a.chunks, cus);
   // A few rows or columns over a multiple of 256 can cost a round of tiles of their own: they go to
-  // the kernel for few rows, in a launch of theirs (4096 x 4100 x 2048: 39 us whole, 33 cut).
+  // the kernel for few rows, in a launch of theirs (4096 x 4100 x 2048: 37 us whole, 29 cut).
   const int64_t over_m = a.m % 256 <= 64 ? a.m % 256 : 0, over_n = a.n % 256 <= 64 ? a.n % 256 : 0;
   if (whole.cut <= kTiles128 && (over_m || over_n) && a.m > 256 && a.n > 256 &&
       std::max(a.m, a.n) <= kMostFewRows) {

@@ -265,7 +265,7 @@ template <typename T>
 constexpr int kMoveRows = sizeof(T) == 2 ? 2 : 1;
 // waves of a workgroup of quantize_columns, side by side along the rows of x: unaligned rows have
 // lines that two of them read (16385 x 4100 bfloat16: 49 us with one, 38 with four, 42 with eight)
-constexpr int kColumnWaves = 4;  // row sets per workgroup: as many loads in flight per thread
+constexpr int kColumnWaves = 4;
 
 // Largest of the four lanes of a quad, in all four.
 __device__ __forceinline__ unsigned quad_max(unsigned v) {
@@ -277,8 +277,9 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
 
 // Blocks along a row.  A thread takes 8 columns, a quad a block, 16 lanes a chunk of 128 columns;
 // the workgroup's 16 chunk slots are 2^tc across and 16 / 2^tc rows.  Bound by the bytes of x:
-// 250000 x 512 doubles 190 us, 5.7 TB/s; 16385 x 4100 bfloat16 28 us, 6.2 TB/s, with dropout 44 (there
-// by the generator's 60 instructions per 8 values).
+// 250000 x 512 doubles 190 us call after call, 5.7 TB/s (233 in turn with the way back to floats);
+// 16385 x 4100 bfloat16 28 us, 6.2 TB/s, with dropout 44 (there by the generator's 60 instructions per
+// 8 values).
 template <typename T, bool DROP>
 __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
   typedef typename Elem<T>::wide W;
@@ -316,17 +317,17 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows(QuantArgs a) {
       s = scale_byte(half_mag_bits<T>(quad_max(top)), 0.f);
       w = s == 255u ? 0u : encode_pairs<T>(pairs, scale_value(s));
     } else {
-    W v[8];
-    const unsigned drop = DROP ? marks_of_pieces<T>(drop_marks(a.mask, group, mask_row(a.mask, r)), l4) : 0u;
+      W v[8];
+      const unsigned drop = DROP ? marks_of_pieces<T>(drop_marks(a.mask, group, mask_row(a.mask, r)), l4) : 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = Elem<T>::up(in[u].v[i]);
-      if (DROP && (drop >> 4 * i & 1)) v[i] = W(0);
-      const unsigned b = mag_bits(v[i]);
-      top = b > top ? b : top;
-    }
-    s = scale_byte(quad_max(top), W(0));
-    w = codes_in_order<T>(s == 255u ? 0u : encode8(v, s), l4);
+      for (int i = 0; i < 8; ++i) {
+        v[i] = Elem<T>::up(in[u].v[i]);
+        if (DROP && (drop >> 4 * i & 1)) v[i] = W(0);
+        const unsigned b = mag_bits(v[i]);
+        top = b > top ? b : top;
+      }
+      s = scale_byte(quad_max(top), W(0));
+      w = codes_in_order<T>(s == 255u ? 0u : encode8(v, s), l4);
     }
     if (c / 2 < a.ldc && chunk < a.chunks)
       *reinterpret_cast<unsigned*>(a.codes + r * a.ldc + c / 2) = w;
@@ -365,7 +366,8 @@ __device__ __forceinline__ void put_column_block(const QuantArgs& a, const Pack<
 // bytes of a row of x and the 8 groups of lanes 256 rows, so that a result row is written in
 // pieces of 128 bytes.  The columns behind the last whole V are left to a wave of their own (the
 // last of a tile row), where a thread takes one column.  250000 x 512 doubles 211 us, 5.2 TB/s;
-// 16385 x 4100 bfloat16 38 us, with dropout 40: two waves to a SIMD, their tiles fill the registers.
+// 16385 x 4100 bfloat16 38 us, with dropout 40 (48 in turn with the way back): two waves to a SIMD,
+// their tiles fill the registers.
 template <typename T, bool DROP>
 __global__ __launch_bounds__(64 * kColumnWaves, 2) void quantize_columns(QuantArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -478,7 +480,7 @@ struct DequantArgs {
 };
 
 // The same layout the other way: a lane loads the codes of 8 columns, the quad deals them out.  Bound
-// by the bytes written: 250000 x 512 floats 120 us, 4.8 TB/s (a fill alone 6.9, a copy 5.1).
+// by the bytes written: 250000 x 512 floats 115 to 120 us, 4.8 to 5.0 TB/s (a fill alone 6.9, a copy 5.1).
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void dequantize_rows(DequantArgs a) {
   typedef typename Elem<T>::wide W;
@@ -779,7 +781,7 @@ int plr_mxfp_quantize(int device_id, void* hip_stream, const void* dx, unsigned 
   a.tc_log2 = 0;
   unsigned grid = 0;
   if (tr) {
-    const int64_t v = 16 / (int64_t)size;  // columns a thread takes; what is over has its own workgroups
+    const int64_t v = 16 / (int64_t)size;  // columns a thread takes; what is over has its own waves
     const int64_t x = ceil_div(ceil_div(d / v, 8) + (d % v != 0), kColumnWaves), y = ceil_div(a.chunks * 4, 8);
     if (!fits_launch(x, y, 64 * kColumnWaves)) return c.bad(PLR_ERR_INVALID, "matrix too large for one launch");
     a.nbx = (unsigned)x;

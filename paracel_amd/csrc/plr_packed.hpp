@@ -3,8 +3,9 @@
 // per value instead of 8, optionally with dropout of the values, arithmetic in 64 bits.
 //
 // Bound by instructions, not bytes: a value costs two multiply-adds in 64 bits and 1.5
-// conversions for each of them, with dropout also an eighth of a generator call.  200000 x 1000: 65 us,
-// of which the 6.9 instructions a value that are issued take 39; with dropout 106 and 80 (14.4).
+// conversions for each of them, with dropout also an eighth of a generator call.  200000 x 1000: 62 to
+// 65 us, of which the 6.9 instructions a value that are issued take 39; with dropout 102 to 113 and 80
+// (14.4).
 //
 // A thread owns one block of 32 columns: its gradient sums stay in registers for the kernel's
 // lifetime, theta is in LDS, a row's 32 values are 16 bytes.  A workgroup lays G = threads /
